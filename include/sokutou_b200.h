@@ -53,7 +53,7 @@ extern "C" {
 
 /* device error word values (sk_device_error) */
 #define SK_DEVERR_NONE 0
-#define SK_DEVERR_POS_RANGE 1     /* decode: pos_ptr[0] + pos_add outside [0, max_len) */
+#define SK_DEVERR_POS_RANGE 1     /* a position or row count read from device memory is out of its range */
 #define SK_DEVERR_TIMEOUT 2       /* a bounded mbarrier wait ran out */
 #define SK_DEVERR_BOUNDS 3        /* bounds-checked build only: an index outside its buffer (access skipped) */
 
@@ -352,6 +352,125 @@ SK_API int sk_decode_attention_noalloc(const float* qkv, const float* qn, const 
                         const float* rope, void* Kc, void* Vc,
                         const long long* pos_ptr, int pos_add, int max_len, int nq, int nkv, int hd,
                         float* out, int cache_dtype, void* stream);
+
+/* ---- 3. Decode over shared prefixes and bounded caches ------------------------------------------ */
+
+/*
+ * What sk_decode_attention_shared needs besides the step's own activations: a HOST struct, filled once
+ * for a layer (it is read during the call and not kept). Strides count elements; the hd elements of a
+ * row are contiguous. K/V pointers 16-byte aligned, K/V strides multiples of 16 bytes.
+ */
+typedef struct SkSharedDecode {
+  const void* Kp;                /* shared prefix keys, row p of head h at h*prefix_head_stride + p*prefix_row_stride */
+  const void* Vp;
+  long long prefix_head_stride;
+  long long prefix_row_stride;   /* >= hd */
+  void* Kc;                      /* own rows: row j of head h of request r at r*request_stride + h*head_stride + */
+  void* Vc;                      /*   j*row_stride                                                              */
+  long long request_stride;
+  long long head_stride;
+  long long row_stride;          /* >= hd */
+  float* mass;                   /* running attention weight per own row (see below); NULL: not kept */
+  long long mass_request_stride;
+  long long mass_head_stride;
+  const float* rope;             /* fp32 [rope_len][hd] = [cos(hd/2) | sin(hd/2)], as sk_decode_attention */
+  const long long* pos;          /* device [R]: position of the new token; negative: the slot is idle */
+  const long long* rows;         /* device [R]: own rows held before this step; NULL: pos[r] - prefix_len */
+  void* workspace;               /* sk_decode_shared_workspace_bytes() bytes, 256-byte aligned, any contents */
+  size_t ws_bytes;
+  long long qkv_stride;          /* elements between two requests' rows of qkv and of out */
+  long long out_stride;
+  int R, nq, nkv, hd;
+  int prefix_len;                /* P: rows of the shared prefix (0: none, Kp and Vp unused) */
+  int max_len;                   /* own rows a request's cache can hold */
+  int rope_len;
+  int cache_dtype;               /* Kp, Vp, Kc, Vc: SK_BF16 or SK_F32 */
+  int qkv_dtype, out_dtype;      /* SK_F32, or SK_BF16 with bf16 caches */
+  float eps;
+  float scale;                   /* softmax scale; <= 0 selects 1/sqrt(hd) */
+} SkSharedDecode;
+
+/* Bytes of workspace sk_decode_attention_shared needs for this struct's sizes, cache_dtype and mass
+ * (NULL or not); 0 for sizes it refuses. */
+SK_API size_t sk_decode_shared_workspace_bytes(const SkSharedDecode* d);
+
+/*
+ * One decode step of one layer for R requests whose caches all continue the same prefix (one voice
+ * prompt, one system prompt): the prefix's keys and values are read once for all requests together, each
+ * request's own rows once. No counterpart in the reference, which serves one request at a time
+ * (README.md:186); per request the arithmetic of its `attn` kernel (qwen3/kernels.py:338-414).
+ *
+ * For every request r with pos[r] >= 0, n = rows[r] (or pos[r] - P) own rows and group g = nq / nkv:
+ *   - q heads RMS-normalised (x qn) and rotated at pos[r]; the new k normalised (x kn) and rotated, k and
+ *     v stored in the cache dtype as own row n;
+ *   - out[r] = softmax(q.k * scale) . v over the prefix rows [0, P) and the own rows [0, n];
+ *   - with mass: mass[r][h][j] += sum over the g query heads of head h of row j's softmax weight for
+ *     j < n, and mass[r][h][n] = that sum for the new row (whatever was there before).
+ * pos[r] and n are separate so that a cache whose rows were evicted (sk_cache_evict) goes on at its true
+ * position. A negative pos[r] marks an idle slot: nothing of it is read (but qkv, unused) or written. A
+ * position outside [0, rope_len) or a row outside [0, max_len) sets SK_DEVERR_POS_RANGE and is treated
+ * as idle.
+ *
+ *   qkv      : [R][(nq + 2*nkv) * hd] = [q heads | k heads | v heads], qkv_stride between rows
+ *   qn, kn   : fp32 [hd]
+ *   out      : [R][nq * hd], out_stride between rows
+ *   Sums, softmax statistics and the accumulated output are fp32. bf16 caches run on the tensor cores
+ *   with q as a sum of two bf16 terms (2^-17 of q) and the weights rounded to bf16, or with an fp32 `out`
+ *   split into two bf16 terms as well.
+ *   nq a multiple of nkv with at most 8 query heads per key/value head; hd 64 or 128; R <= 1024.
+ * Launches kernels only (capturable). Two calls that may run at the same time need two workspaces. The
+ * requests' caches, masses and outputs must not overlap. Results do not depend on scheduling.
+ */
+SK_API int sk_decode_attention_shared(const SkSharedDecode* d, const void* qkv, const float* qn, const float* kn,
+                                      void* out, void* stream);
+
+/*
+ * What sk_cache_evict works on: caches of N layers x R requests x nkv heads. A HOST struct. Strides count
+ * elements in the order layer, request, head, row (the row stride of mass is 1); the hd elements of a row
+ * are contiguous. K/V pointers 16-byte aligned, K/V strides multiples of 16 bytes.
+ */
+typedef struct SkCacheEvict {
+  const void* K;              /* source */
+  const void* V;
+  const float* mass;
+  long long kv_stride[4];
+  long long mass_stride[3];
+  void* K_out;                /* destination; all three may be the source itself (in place) */
+  void* V_out;
+  float* mass_out;
+  long long kv_out_stride[4];
+  long long mass_out_stride[3];
+  const long long* rows;      /* device [R]: rows each request's caches hold */
+  long long* rows_out;        /* device [R]: rows they hold afterwards; may be `rows` */
+  void* workspace;            /* sk_cache_evict_workspace_bytes() bytes, 256-byte aligned, any contents */
+  size_t ws_bytes;
+  int N, R, nkv, hd;
+  int max_len;                /* rows a source cache can hold */
+  int max_len_out;            /* rows a destination can hold, >= keep */
+  int keep, first, recent;
+  int cache_dtype;            /* SK_BF16 or SK_F32 */
+} SkCacheEvict;
+
+/* Bytes of workspace sk_cache_evict needs for this struct's sizes; 0 for sizes it refuses. */
+SK_API size_t sk_cache_evict_workspace_bytes(const SkCacheEvict* d);
+
+/*
+ * Brings every cache of every request down to at most `keep` rows by the accumulated attention weights
+ * that sk_decode_attention_shared keeps. A cache of n = rows[r] > keep rows keeps its `first` first rows,
+ * its `recent` last rows and, of the rows between, the keep - first - recent with the greatest mass: the
+ * lowest row first among equals, a NaN below every number. The kept rows move to rows [0, keep) in their
+ * order, K, V and mass alike; each layer and head keeps its own choice (keys are stored rotated, so a row
+ * may move). rows_out[r] = keep. A request with n <= keep keeps everything (copied when the destination
+ * is another buffer), rows_out[r] = n; a negative n marks an idle slot, untouched, rows_out[r] = n.
+ * Destination rows from rows_out[r] on are left as they were. n > max_len sets SK_DEVERR_POS_RANGE and is
+ * treated as idle. No counterpart in the reference, whose caches end at max_len.
+ *
+ * Destination and source are either the same buffers with the same strides, or the address ranges that
+ * they span do not meet (else SK_ERR_INVALID_ARG).
+ * 0 <= first, recent; first + recent <= keep; 1 <= keep <= max_len, max_len_out; hd 64 or 128.
+ * Launches kernels only (capturable); two calls that may run at the same time need two workspaces.
+ */
+SK_API int sk_cache_evict(const SkCacheEvict* d, void* stream);
 
 #ifdef __cplusplus
 }

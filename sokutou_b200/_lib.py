@@ -43,6 +43,10 @@ SIGNATURES = {
     "sk_decode_attention_grouped": (_I, [_P, _I, _I, _I, _I, _I, _I, _I, _P]),
     "sk_decode_attention_block": (_I, [_P, _P, _F, _P, _P, _P, _F, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _I, _I, _I,
                                        _P, _SZ, _I, _P]),
+    "sk_decode_shared_workspace_bytes": (_SZ, [_P]),
+    "sk_decode_attention_shared": (_I, [_P, _P, _P, _P, _P, _P]),
+    "sk_cache_evict_workspace_bytes": (_SZ, [_P]),
+    "sk_cache_evict": (_I, [_P, _P]),
 }
 
 
@@ -54,6 +58,27 @@ class SkDecodeRequest(ctypes.Structure):
 
 
 assert ctypes.sizeof(SkDecodeRequest) == 80
+
+
+class SkSharedDecode(ctypes.Structure):
+    """include/sokutou_b200.h SkSharedDecode: the fixed arguments of sk_decode_attention_shared."""
+    _fields_ = [("Kp", _P), ("Vp", _P), ("prefix_head_stride", _LL), ("prefix_row_stride", _LL), ("Kc", _P), ("Vc", _P),
+                ("request_stride", _LL), ("head_stride", _LL), ("row_stride", _LL), ("mass", _P),
+                ("mass_request_stride", _LL), ("mass_head_stride", _LL), ("rope", _P), ("pos", _P), ("rows", _P),
+                ("workspace", _P), ("ws_bytes", _SZ), ("qkv_stride", _LL), ("out_stride", _LL), ("R", _I), ("nq", _I),
+                ("nkv", _I), ("hd", _I), ("prefix_len", _I), ("max_len", _I), ("rope_len", _I), ("cache_dtype", _I),
+                ("qkv_dtype", _I), ("out_dtype", _I), ("eps", _F), ("scale", _F)]
+
+
+class SkCacheEvict(ctypes.Structure):
+    """include/sokutou_b200.h SkCacheEvict: the arguments of sk_cache_evict."""
+    _fields_ = [("K", _P), ("V", _P), ("mass", _P), ("kv_stride", _LL * 4), ("mass_stride", _LL * 3), ("K_out", _P),
+                ("V_out", _P), ("mass_out", _P), ("kv_out_stride", _LL * 4), ("mass_out_stride", _LL * 3), ("rows", _P),
+                ("rows_out", _P), ("workspace", _P), ("ws_bytes", _SZ), ("N", _I), ("R", _I), ("nkv", _I), ("hd", _I),
+                ("max_len", _I), ("max_len_out", _I), ("keep", _I), ("first", _I), ("recent", _I), ("cache_dtype", _I)]
+
+
+assert ctypes.sizeof(SkSharedDecode) == 200 and ctypes.sizeof(SkCacheEvict) == 232
 
 _lib = None
 

@@ -1,0 +1,464 @@
+// Decode attention of many requests behind one shared prefix: the CUDA-core kernel over key tiles (fp32
+// caches), the kernel that joins the partials with the step's own token, and the entry points. The work
+// split and the workspace are described in shared_decode.cuh.
+#include "shared_decode.cuh"
+
+namespace sk {
+namespace shared {
+
+template <typename T>
+struct Elem;
+template <>
+struct Elem<__nv_bfloat16> {
+  static __device__ __forceinline__ float ld(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+  static __device__ __forceinline__ void ld4(const __nv_bfloat16* p, float (&x)[4]) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    x[0] = __uint_as_float(v.x << 16), x[1] = __uint_as_float(v.x & 0xffff0000u);
+    x[2] = __uint_as_float(v.y << 16), x[3] = __uint_as_float(v.y & 0xffff0000u);
+  }
+  static __device__ __forceinline__ __nv_bfloat16 st(float f) { return __float2bfloat16_rn(f); }
+  static __device__ __forceinline__ float rnd(float f) { return __bfloat162float(__float2bfloat16_rn(f)); }
+};
+template <>
+struct Elem<float> {
+  static __device__ __forceinline__ float ld(const float* p) { return *p; }
+  static __device__ __forceinline__ void ld4(const float* p, float (&x)[4]) {
+    const float4 v = *reinterpret_cast<const float4*>(p);
+    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+  }
+  static __device__ __forceinline__ float st(float f) { return f; }
+  static __device__ __forceinline__ float rnd(float f) { return f; }
+};
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void griddep_launch_dependents() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+// 16 bytes to shared memory; `keep` false writes zeros (and reads nothing).
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool keep) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(keep ? 16 : 0)
+               : "memory");
+}
+
+// ---- key tiles on the CUDA cores -------------------------------------------------------------------
+// One CTA of 128 threads walks its share of 64-key tiles, up to 16 query rows against each: K and V rows
+// by 16-byte asynchronous copies, scores by one thread per (key, row parity), an online softmax per row,
+// P·V by one thread per output column with the rows' sums in registers.
+constexpr int kSimtThreads = 128;
+
+template <typename T, int HD>
+struct SimtSmem {
+  static constexpr int KT = CutSimt::KT, RT = CutSimt::RT;
+  static constexpr int PITCH = HD + 16 / (int)sizeof(T);  // an odd number of 16-byte units: no bank conflicts
+  static constexpr int OFF_K = RT * HD * 4;
+  static constexpr int OFF_V = OFF_K + KT * PITCH * (int)sizeof(T);
+  static constexpr int OFF_P = OFF_V + KT * PITCH * (int)sizeof(T);
+  static constexpr int OFF_ST = OFF_P + RT * KT * 4;      // m, l, alpha per row
+  static constexpr int OFF_CUM = OFF_ST + 3 * RT * 4;
+  static __host__ __device__ int bytes(int R) { return OFF_CUM + (R + 1) * 4; }
+};
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kSimtThreads) tiles_simt_kernel(const Params p) {
+  using S = SimtSmem<T, HD>;
+  constexpr int KT = S::KT, RT = S::RT, E = HD / 32, NG = kSimtThreads / HD;
+  extern __shared__ __align__(128) uint8_t smem[];
+  float* Qs = reinterpret_cast<float*>(smem);
+  T* Ks = reinterpret_cast<T*>(smem + S::OFF_K);
+  T* Vs = reinterpret_cast<T*>(smem + S::OFF_V);
+  float* Ps = reinterpret_cast<float*>(smem + S::OFF_P);
+  float* m_s = reinterpret_cast<float*>(smem + S::OFF_ST);
+  float* l_s = m_s + RT;
+  float* a_s = l_s + RT;
+  int* cum = reinterpret_cast<int*>(smem + S::OFF_CUM);
+  __shared__ int any_s;
+  const int t = threadIdx.x, lane = t & 31, w = t >> 5, c = blockIdx.x;
+
+  griddep_wait();
+  griddep_launch_dependents();
+  if (w == 0) {
+    const bool any = scan_tiles<KT>(p, cum, c == 0);
+    if (lane == 0) any_s = any;
+  }
+  __syncthreads();
+  if (c == 0)
+    for (int r = t; r <= p.R; r += kSimtThreads) p.cum[r] = cum[r];
+  const Tiles tl = tiles_of<CutSimt>(p, cum[p.R], any_s);
+  const long long end = share_begin(tl, c + 1);
+
+  for (long long tile = share_begin(tl, c); tile < end;) {
+    const Segment sg = segment_at<CutSimt>(p, tl, cum, tile, end);
+    tile += sg.t1 - sg.t0;
+    const int row0 = sg.prefix ? sg.r * RT : 0;
+    const int n_rows = sg.prefix ? min(RT, p.R * p.g - row0) : p.g;
+    const T* Kb = sg.prefix ? reinterpret_cast<const T*>(p.Kp) + sg.kvh * p.prefix_head_stride
+                            : reinterpret_cast<const T*>(p.Kc) + sg.r * p.request_stride + sg.kvh * p.head_stride;
+    const T* Vb = sg.prefix ? reinterpret_cast<const T*>(p.Vp) + sg.kvh * p.prefix_head_stride
+                            : reinterpret_cast<const T*>(p.Vc) + sg.r * p.request_stride + sg.kvh * p.head_stride;
+    const long long pitch = sg.prefix ? p.prefix_row_stride : p.row_stride;
+
+    for (int i = w; i < n_rows; i += kSimtThreads / 32) {
+      const int r = sg.prefix ? (row0 + i) / p.g : sg.r, h = sg.prefix ? (row0 + i) % p.g : i;
+      float x[E] = {};
+      bool bad = false;
+      if (own_rows(p, r, &bad) >= 0) {
+        load_row<HD>(p.qkv, r * p.qkv_stride + (long long)(sg.kvh * p.g + h) * HD, p.qkv_bf16, x);
+        norm_rotate<HD>(x, p.qn, p.rope + p.pos[r] * HD, p.eps);
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] *= p.q_scale;
+      }
+      store_vec<E>(Qs + i * HD + lane * E, x);
+    }
+    if (t < RT) {
+      m_s[t] = -INFINITY;
+      l_s[t] = 0.f;
+    }
+    float acc[RT / NG] = {};
+    const int d = t % HD, grp = t / HD;
+
+    for (int tt = sg.t0; tt < sg.t1; ++tt) {
+      const int j0 = tt * KT, nk = min(KT, sg.n_keys - j0);
+      __syncthreads();  // Q in place; the last tile's K, V and P read
+      constexpr int U = HD * (int)sizeof(T) / 16;  // 16-byte units per row
+      for (int i = t; i < KT * U; i += kSimtThreads) {
+        const int j = i / U, u = i % U;
+        const long long at = (long long)(j0 + (j < nk ? j : 0)) * pitch + u * (16 / (int)sizeof(T));
+        cp_async16(Ks + j * S::PITCH + u * (16 / (int)sizeof(T)), Kb + at, j < nk);
+        cp_async16(Vs + j * S::PITCH + u * (16 / (int)sizeof(T)), Vb + at, j < nk);
+      }
+      asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+      __syncthreads();
+      {  // scores: rows half, half + 2, ... against one key
+        const int j = t % KT, half = t / KT;
+        float s[RT / 2] = {};
+#pragma unroll 4
+        for (int k4 = 0; k4 < HD; k4 += 4) {
+          float kv[4];
+          Elem<T>::ld4(Ks + j * S::PITCH + k4, kv);
+#pragma unroll
+          for (int i = 0; i < RT / 2; ++i) {
+            if (2 * i + half >= n_rows) break;
+            const float4 q = *reinterpret_cast<const float4*>(Qs + (2 * i + half) * HD + k4);
+            s[i] += q.x * kv[0] + q.y * kv[1] + q.z * kv[2] + q.w * kv[3];
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < RT / 2; ++i) {
+          const int row = 2 * i + half;
+          if (row < n_rows) {
+            Ps[row * KT + j] = j < nk ? s[i] : -INFINITY;
+            if (!sg.prefix && p.mass && j < nk)
+              p.sc[((long long)sg.r * p.nq + sg.kvh * p.g + row) * p.sc_stride + j0 + j] = s[i];
+          }
+        }
+      }
+      __syncthreads();
+      for (int i = w; i < n_rows; i += kSimtThreads / 32) {
+        const float s0 = Ps[i * KT + lane], s1 = Ps[i * KT + 32 + lane];
+        const float m_old = m_s[i], m = fmaxf(m_old, warp_max(fmaxf(s0, s1)));
+        const float use = m == -INFINITY ? 0.f : m;  // every score so far -inf: weights 0, not NaN
+        const float p0 = ex2_approx(s0 - use), p1 = ex2_approx(s1 - use), a = ex2_approx(m_old - use);
+        const float l = warp_sum(p0 + p1);
+        Ps[i * KT + lane] = p0;
+        Ps[i * KT + 32 + lane] = p1;
+        if (lane == 0) {
+          m_s[i] = m;
+          l_s[i] = l_s[i] * a + l;
+          a_s[i] = a;
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < RT / NG; ++i)
+        if (i * NG + grp < n_rows) acc[i] *= a_s[i * NG + grp];
+#pragma unroll 2
+      for (int j = 0; j < KT; j += 4) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = Elem<T>::ld(Vs + (j + e) * S::PITCH + d);
+#pragma unroll
+        for (int i = 0; i < RT / NG; ++i) {
+          if (i * NG + grp >= n_rows) break;
+          const float4 q = *reinterpret_cast<const float4*>(Ps + (i * NG + grp) * KT + j);
+          acc[i] += q.x * v[0] + q.y * v[1] + q.z * v[2] + q.w * v[3];
+        }
+      }
+    }
+    const long long slot = (long long)c + sg.item;
+    float* o = sg.prefix ? p.po + slot * RT * HD : p.oo + slot * p.g * HD;
+    float* ml = sg.prefix ? p.pml + slot * RT * 2 : p.oml + slot * p.g * 2;
+#pragma unroll
+    for (int i = 0; i < RT / NG; ++i)
+      if (i * NG + grp < n_rows) o[(i * NG + grp) * HD + d] = acc[i];
+    if (t < n_rows) {
+      ml[2 * t] = m_s[t];
+      ml[2 * t + 1] = l_s[t];
+    }
+    __syncthreads();  // Q and the statistics are free for the next segment
+  }
+}
+
+// ---- joining the partials ---------------------------------------------------------------------------
+// One CTA per (request, key/value head): the new token's k and v (normalised, rotated, stored as own row
+// n, attended as the cache holds them), the partials of the prefix and of the own rows, out, and, a chunk
+// of kMassChunk rows per CTA of grid row y, the weights 2^(s - M) / L added to the mass. An item's
+// partials lie in the slots of the CTAs from the one that holds its first tile to the one that holds its
+// last. The 8 warps are shared out over the heads of the group; a warp reads whole output rows.
+constexpr int kJoinThreads = 256, kMassChunk = 1024;
+
+template <class Cut, typename T, int HD>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
+  constexpr int E = HD / 32, OQ = Cut::OQ, RT = Cut::RT;
+  __shared__ float snew_s[kMaxGroup], M_s[kMaxGroup], iL_s[kMaxGroup];
+  __shared__ __align__(16) float red_s[kJoinThreads / 32][HD];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int r = blockIdx.x / p.nkv, kvh = blockIdx.x % p.nkv;
+  griddep_wait();  // every thread, before any exit: the kernel after this one relies on it
+  griddep_launch_dependents();
+  bool bad = false;
+  const int n = own_rows(p, r, &bad);
+  if (n < 0 || (blockIdx.y > 0 && (int)blockIdx.y * kMassChunk >= n)) return;
+
+  const int per = max(1, (kJoinThreads / 32) / p.g), h = w / per, sub = w % per;  // warps per head
+  const float* turn = p.rope + p.pos[r] * HD;
+  float v[E] = {};
+  float acc[E] = {};
+  float w_new = 0.f;
+  if (h < p.g) {
+    float q[E], k[E];
+    const long long base = r * p.qkv_stride;
+    load_row<HD>(p.qkv, base + (long long)(kvh * p.g + h) * HD, p.qkv_bf16, q);
+    load_row<HD>(p.qkv, base + (long long)(p.nq + kvh) * HD, p.qkv_bf16, k);
+    load_row<HD>(p.qkv, base + (long long)(p.nq + p.nkv + kvh) * HD, p.qkv_bf16, v);
+    norm_rotate<HD>(q, p.qn, turn, p.eps);
+    norm_rotate<HD>(k, p.kn, turn, p.eps);
+    float dot = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      k[e] = Elem<T>::rnd(k[e]);
+      v[e] = Elem<T>::rnd(v[e]);
+      dot += q[e] * p.q_scale * k[e];
+    }
+    const float s_new = warp_sum(dot);
+    if (w == 0 && blockIdx.y == 0) {
+      const long long at = r * p.request_stride + kvh * p.head_stride + n * p.row_stride + lane * E;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        reinterpret_cast<T*>(p.Kc)[at + e] = Elem<T>::st(k[e]);
+        reinterpret_cast<T*>(p.Vc)[at + e] = Elem<T>::st(v[e]);
+      }
+    }
+    // where this head's partials lie
+    const Tiles tl = tiles_of<Cut>(p, p.cum[p.R], true);
+    const int i = r * p.g + h, rt = i / RT, il = i - rt * RT;
+    const bool split = OQ > 1 && min(RT, p.R * p.g - rt * RT) <= RT / OQ;  // the tile's rows ran once per key quarter
+    const int pq = split ? OQ : 1, ip = kvh * tl.nrt + rt;
+    int pc = 0, np = 0;
+    if (tl.tp > 0) {
+      pc = share_of(tl, (long long)ip * tl.tp);
+      np = (share_of(tl, (long long)(ip + 1) * tl.tp - 1) - pc + 1) * pq;
+    }
+    const int tr = p.cum[r + 1] - p.cum[r], io = r * p.nkv + kvh;
+    int oc = 0, no = 0;
+    if (tr > 0) {
+      const long long first = tl.n_prefix + (long long)p.cum[r] * p.nkv + (long long)kvh * tr;
+      oc = share_of(tl, first);
+      no = (share_of(tl, first + tr - 1) - oc + 1) * OQ;
+    }
+    auto place = [&](int x) -> long long {  // partial row of partial x, own rows counted from np
+      if (x < np) return ((long long)(pc + x / pq) + ip) * RT + il + (x % pq) * (RT / OQ);
+      x -= np;
+      return (((long long)(oc + x / OQ) + io) * OQ + x % OQ) * p.g + h;
+    };
+    float M = s_new;
+    for (int x = lane; x < np + no; x += 32) M = fmaxf(M, __ldcg((x < np ? p.pml : p.oml) + 2 * place(x)));
+    M = warp_max(M);
+    float L = 0.f;
+    for (int x = lane; x < np + no; x += 32) {
+      const float2 ml = __ldcg(reinterpret_cast<const float2*>((x < np ? p.pml : p.oml) + 2 * place(x)));
+      L += ml.y * ex2_approx(ml.x - M);
+    }
+    w_new = ex2_approx(s_new - M);
+    L = warp_sum(L) + w_new;
+    if (sub == 0 && lane == 0) {
+      snew_s[h] = s_new;
+      M_s[h] = M;
+      iL_s[h] = 1.f / L;
+    }
+    if (blockIdx.y == 0) {
+#pragma unroll 4
+      for (int x = sub; x < np + no; x += per) {
+        const long long at = place(x);
+        const float wt = ex2_approx(__ldcg((x < np ? p.pml : p.oml) + 2 * at) - M);
+        float o[E];
+        load_vec<E>((x < np ? p.po : p.oo) + at * HD + lane * E, o);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += wt * o[e];
+      }
+      store_vec<E>(red_s[w] + lane * E, acc);
+    }
+  }
+  __syncthreads();
+  if (blockIdx.y == 0 && h < p.g && sub == 0) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] += w_new * v[e];
+    for (int x = 1; x < per; ++x) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] += red_s[w + x][lane * E + e];
+    }
+    const long long at = r * p.out_stride + (long long)(kvh * p.g + h) * HD + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] *= iL_s[h];
+    if (p.out_bf16) {
+      __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(p.out) + at;
+#pragma unroll
+      for (int e = 0; e < E; e += 2)
+        *reinterpret_cast<__nv_bfloat162*>(o + e) = __floats2bfloat162_rn(acc[e], acc[e + 1]);
+    } else {
+      store_vec<E>(reinterpret_cast<float*>(p.out) + at, acc);
+    }
+  }
+  if (!p.mass) return;
+  float* mass = p.mass + r * p.mass_request_stride + kvh * p.mass_head_stride;
+  const float* sc = p.sc + ((long long)r * p.nq + kvh * p.g) * p.sc_stride;
+  const int j0 = blockIdx.y * kMassChunk, j1 = min(n, j0 + kMassChunk);
+  for (int j = j0 + threadIdx.x; j < j1; j += kJoinThreads) {
+    float a = 0.f;
+    for (int x = 0; x < p.g; ++x) a += ex2_approx(__ldcg(sc + x * p.sc_stride + j) - M_s[x]) * iL_s[x];
+    mass[j] += a;
+  }
+  if (blockIdx.y == 0 && threadIdx.x == 0) {
+    float a = 0.f;
+    for (int x = 0; x < p.g; ++x) a += ex2_approx(snew_s[x] - M_s[x]) * iL_s[x];
+    mass[n] = a;
+  }
+}
+
+// ---- host -----------------------------------------------------------------------------------------
+static int check_sizes(const SkSharedDecode* d) {
+  if (!d) return SK_ERR_INVALID_ARG;
+  if (d->cache_dtype != SK_BF16 && d->cache_dtype != SK_F32) return SK_ERR_UNSUPPORTED;
+  if (d->hd != 64 && d->hd != 128) return SK_ERR_UNSUPPORTED;
+  if (d->R < 1 || d->nkv < 1 || d->nq < 1 || d->prefix_len < 0 || d->max_len < 1 || d->rope_len < 1)
+    return SK_ERR_INVALID_ARG;
+  if (d->nq % d->nkv != 0 || d->nq / d->nkv > kMaxGroup || d->R > kMaxRequests || d->nkv > 1024)
+    return SK_ERR_UNSUPPORTED;
+  if (d->prefix_len > (1 << 30) || d->max_len > (1 << 30)) return SK_ERR_UNSUPPORTED;
+  return SK_OK;
+}
+
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+template <class Cut, typename T, int HD>
+static int launch_join(const Params& p, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.R * p.nkv), (unsigned)(p.mass ? (p.max_len + kMassChunk - 1) / kMassChunk : 1));
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, join_kernel<Cut, T, HD>, p) == cudaSuccess ? SK_OK : SK_ERR_CUDA;
+}
+
+template <typename T, int HD>
+static int launch_simt(const Params& p, cudaStream_t st) {
+  const int smem = SimtSmem<T, HD>::bytes(p.R);
+  if (cudaFuncSetAttribute(tiles_simt_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return SK_ERR_CUDA;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(CutSimt::G);
+  cfg.blockDim = dim3(kSimtThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, tiles_simt_kernel<T, HD>, p) != cudaSuccess) return SK_ERR_CUDA;
+  return launch_join<CutSimt, T, HD>(p, st);
+}
+
+}  // namespace shared
+}  // namespace sk
+
+extern "C" size_t sk_decode_shared_workspace_bytes(const SkSharedDecode* d) {
+  using namespace sk::shared;
+  if (check_sizes(d) != SK_OK) return 0;
+  return (size_t)ws_layout<CutSimt>(d->R, d->nq, d->nkv, d->hd, d->prefix_len, d->max_len, d->mass != nullptr).bytes;
+}
+
+extern "C" int sk_decode_attention_shared(const SkSharedDecode* d, const void* qkv, const float* qn, const float* kn,
+                                          void* out, void* stream) {
+  using namespace sk::shared;
+  const int rc = check_sizes(d);
+  if (rc != SK_OK) return rc;
+  const int esz = d->cache_dtype == SK_BF16 ? 2 : 4, per16 = 16 / esz, hd = d->hd;
+  const bool q16 = d->qkv_dtype == SK_BF16, o16 = d->out_dtype == SK_BF16;
+  if ((!q16 && d->qkv_dtype != SK_F32) || (!o16 && d->out_dtype != SK_F32)) return SK_ERR_UNSUPPORTED;
+  if ((q16 || o16) && d->cache_dtype != SK_BF16) return SK_ERR_UNSUPPORTED;
+  if (!qkv || !qn || !kn || !out || !d->rope || !d->pos || !d->Kc || !d->Vc) return SK_ERR_INVALID_ARG;
+  if (!aligned16(qkv) || !aligned16(qn) || !aligned16(kn) || !aligned16(out) || !aligned16(d->rope) ||
+      !aligned16(d->Kc) || !aligned16(d->Vc))
+    return SK_ERR_INVALID_ARG;
+  if ((reinterpret_cast<uintptr_t>(d->pos) | reinterpret_cast<uintptr_t>(d->rows)) & 7) return SK_ERR_INVALID_ARG;
+  if (d->row_stride < hd || d->row_stride % per16 || (d->R > 1 && (d->request_stride < hd || d->request_stride % per16)) ||
+      (d->nkv > 1 && (d->head_stride < hd || d->head_stride % per16)))
+    return SK_ERR_INVALID_ARG;
+  if (d->prefix_len > 0) {
+    if (!d->Kp || !d->Vp || !aligned16(d->Kp) || !aligned16(d->Vp)) return SK_ERR_INVALID_ARG;
+    if (d->prefix_row_stride < hd || d->prefix_row_stride % per16 ||
+        (d->nkv > 1 && (d->prefix_head_stride < hd || d->prefix_head_stride % per16)))
+      return SK_ERR_INVALID_ARG;
+  }
+  if (d->R > 1 && (d->qkv_stride < (long long)(d->nq + 2 * d->nkv) * hd || d->qkv_stride % (q16 ? 8 : 4) ||
+                   d->out_stride < (long long)d->nq * hd || d->out_stride % (o16 ? 8 : 4)))
+    return SK_ERR_INVALID_ARG;
+  if (d->mass && ((reinterpret_cast<uintptr_t>(d->mass) & 3) || (d->R > 1 && d->mass_request_stride < 1) ||
+                  (d->nkv > 1 && d->mass_head_stride < 1)))
+    return SK_ERR_INVALID_ARG;
+  const WsLayout w = ws_layout<CutSimt>(d->R, d->nq, d->nkv, hd, d->prefix_len, d->max_len, d->mass != nullptr);
+  if (!d->workspace || (reinterpret_cast<uintptr_t>(d->workspace) & 255) || d->ws_bytes < (size_t)w.bytes)
+    return SK_ERR_WORKSPACE;
+  const int dev = sk_check_device();
+  if (dev != SK_OK) return dev;
+
+  Params p = {};
+  p.Kp = d->Kp, p.Vp = d->Vp;
+  p.prefix_head_stride = d->prefix_head_stride, p.prefix_row_stride = d->prefix_row_stride;
+  p.Kc = d->Kc, p.Vc = d->Vc;
+  p.request_stride = d->request_stride, p.head_stride = d->head_stride, p.row_stride = d->row_stride;
+  p.mass = d->mass, p.mass_request_stride = d->mass_request_stride, p.mass_head_stride = d->mass_head_stride;
+  p.rope = d->rope, p.pos = d->pos, p.rows = d->rows;
+  p.qkv = qkv, p.qn = qn, p.kn = kn, p.out = out;
+  p.qkv_stride = d->qkv_stride, p.out_stride = d->out_stride;
+  p.R = d->R, p.nq = d->nq, p.nkv = d->nkv, p.g = d->nq / d->nkv;
+  p.P = d->prefix_len, p.max_len = d->max_len, p.rope_len = d->rope_len;
+  p.qkv_bf16 = q16, p.out_bf16 = o16;
+  p.eps = d->eps;
+  p.q_scale = (d->scale > 0.f ? d->scale : (hd == 128 ? 0.08838834764831845f : 0.125f)) * kLog2e;
+  uint8_t* ws = reinterpret_cast<uint8_t*>(d->workspace);
+  p.cum = reinterpret_cast<int*>(ws + w.cum);
+  p.po = reinterpret_cast<float*>(ws + w.po), p.pml = reinterpret_cast<float*>(ws + w.pml);
+  p.oo = reinterpret_cast<float*>(ws + w.oo), p.oml = reinterpret_cast<float*>(ws + w.oml);
+  p.sc = reinterpret_cast<float*>(ws + w.sc), p.sc_stride = w.sc_stride;
+  p.err = sk_error_word_ptr();
+  if (!p.err) return SK_ERR_CUDA;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (d->cache_dtype == SK_BF16)
+    return hd == 128 ? launch_simt<__nv_bfloat16, 128>(p, st) : launch_simt<__nv_bfloat16, 64>(p, st);
+  return hd == 128 ? launch_simt<float, 128>(p, st) : launch_simt<float, 64>(p, st);
+}

@@ -11,6 +11,10 @@ Qwen3 talker (qwen3/kernels.py:622-624):
     decode_attention  — one layer's decode step with the reference kernel's argument list
     decode_attention_block — the layer's rms_gemv(qkv) -> attention -> gemv(o) in one launch
     prefill_attention — the prompt's causal attention (qwen3/fast.py:251-263), tensor cores
+Batches behind a shared prefix, and bounded caches (no counterpart in the reference):
+    decode_attention_shared — one decode step of R requests whose caches continue one prefix, the prefix
+                       read once; optionally adds up each row's attention weight
+    cache_evict      — caches brought down to a budget of rows by those weights
 """
 
 from __future__ import annotations
@@ -432,10 +436,218 @@ def prefill_attention(qkv_rows: torch.Tensor, qn: torch.Tensor, kn: torch.Tensor
     return out
 
 
+# ---- decode behind a shared prefix, bounded caches -----------------------------------------------
+
+def _raw_stream(index: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+class SharedDecodePlan:
+    """The checked, fixed part of decode_attention_shared for one layer (see shared_decode_plan). Holds the
+    tensors it points into; read-only once made, so several threads may use it (with a workspace each)."""
+
+    __slots__ = ("desc", "addr", "device", "index", "qkv_shape", "out_shape", "qkv_dtype", "out_dtype", "qkv_stride",
+                 "out_stride", "hd", "keep", "workspace")
+
+
+def shared_decode_workspace(R: int, nq: int, nkv: int, max_len: int, prefix_len: int, device, hd: int = 128,
+                            cache_dtype: torch.dtype = torch.bfloat16, mass: bool = False) -> torch.Tensor:
+    """A workspace for plans of these sizes. Plans whose calls follow one another on a stream (the layers of
+    one stack) may share one; calls that may run at the same time need one each."""
+    d = _lib.SkSharedDecode(R=R, nq=nq, nkv=nkv, hd=hd, prefix_len=prefix_len, max_len=max_len, rope_len=1,
+                            cache_dtype=_dtype_code(cache_dtype), mass=256 if mass else None)
+    n = int(lib().sk_decode_shared_workspace_bytes(ctypes.byref(d)))
+    _need(n > 0, f"unsupported sizes: R={R} nq={nq} nkv={nkv} hd={hd} prefix_len={prefix_len} max_len={max_len}")
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def shared_decode_plan(K: torch.Tensor, V: torch.Tensor, pos: torch.Tensor, rope: torch.Tensor, nq: int, eps: float,
+                       rows: torch.Tensor | None = None, Kp: torch.Tensor | None = None,
+                       Vp: torch.Tensor | None = None, mass: torch.Tensor | None = None, scale: float | None = None,
+                       qkv_dtype: torch.dtype = torch.float32, out_dtype: torch.dtype = torch.float32,
+                       workspace: torch.Tensor | None = None, qkv_stride: int | None = None,
+                       out_stride: int | None = None) -> SharedDecodePlan:
+    """What decode_attention_shared keeps for one layer, checked once.
+
+    K, V: the requests' own caches (R, nkv, max_len, hd), bf16 or fp32, rows contiguous, any strides else;
+    Kp, Vp: the shared prefix (nkv, P, hd) in the same dtype (None: no prefix), any strides else — a slice
+    [:, :P] of another cache will do; pos int64 (R,): position of each request's new token, negative for an
+    idle slot; rows int64 (R,): own rows held (None: pos - P); rope float32 (rope_len, hd); mass float32
+    (R, nkv, max_len): the running attention weight of every own row, or None. scale None: 1/sqrt(hd).
+    qkv_dtype, out_dtype: float32, or bfloat16 with bf16 caches. qkv_stride, out_stride: elements between two
+    requests' rows where they are not packed. workspace: shared_decode_workspace (None: made here).
+    pos, rows, K, V and mass are read at each call, so a captured call goes on as they change."""
+    _need(K.dim() == 4 and K.shape == V.shape and K.stride() == V.stride(), "K and V must be (R, nkv, max_len, hd), laid out alike")
+    R, nkv, max_len, hd = K.shape
+    dt = K.dtype
+    _need(K.is_cuda, "K must be a CUDA tensor")
+    dev = K.device
+    _need(K.stride(3) == 1, "the elements of a cache row must be contiguous")
+    P = 0
+    if (Kp is None) != (Vp is None):
+        raise ValueError("Kp and Vp go together")
+    if Kp is not None:
+        _need(Kp.dim() == 3 and Kp.shape == Vp.shape and Kp.stride() == Vp.stride() and Kp.shape[0] == nkv
+              and Kp.shape[2] == hd, f"Kp and Vp must be ({nkv}, P, {hd}), laid out alike")
+        P = Kp.shape[1]
+        _need(P == 0 or Kp.stride(2) == 1, "the elements of a prefix row must be contiguous")
+    for n, t, want in (("V", V, dt), ("Kp", Kp, dt), ("Vp", Vp, dt), ("rope", rope, torch.float32),
+                       ("pos", pos, torch.int64), ("rows", rows, torch.int64), ("mass", mass, torch.float32)):
+        if t is not None:
+            _need(t.device == dev, f"{n} must be on {dev}")
+            _need(t.dtype == want, f"{n} must be {want}")
+    for n, t in (("pos", pos), ("rows", rows)):
+        _need(t is None or (t.shape == (R,) and t.is_contiguous()), f"{n} must be contiguous ({R},)")
+    _need(rope.dim() == 2 and rope.shape[1] == hd and rope.is_contiguous(), f"rope must be contiguous (rope_len, {hd})")
+    if mass is not None:
+        _need(mass.shape == (R, nkv, max_len) and (mass.stride(2) == 1 or max_len == 1),
+              f"mass must be ({R}, {nkv}, {max_len}), its rows contiguous")
+    wide = (nq + 2 * nkv) * hd
+    code = _dtype_code(dt)
+    if workspace is None:
+        workspace = shared_decode_workspace(R, nq, nkv, max_len, P, dev, hd, dt, mass is not None)
+    _need(workspace.device == dev and workspace.is_contiguous(), f"workspace must be contiguous on {dev}")
+    p = SharedDecodePlan()
+    ms = (0, 0) if mass is None else mass.stride()[:2]
+    p.desc = _lib.SkSharedDecode(
+        Kp=_ptr(Kp) if P else None, Vp=_ptr(Vp) if P else None, prefix_head_stride=Kp.stride(0) if P else 0,
+        prefix_row_stride=(Kp.stride(1) if P > 1 else hd) if P else 0, Kc=_ptr(K), Vc=_ptr(V),
+        request_stride=K.stride(0), head_stride=K.stride(1), row_stride=K.stride(2) if max_len > 1 else hd,
+        mass=_ptr(mass) or None, mass_request_stride=ms[0], mass_head_stride=ms[1], rope=_ptr(rope), pos=_ptr(pos),
+        rows=_ptr(rows) or None, workspace=_ptr(workspace), ws_bytes=workspace.numel() * workspace.element_size(),
+        qkv_stride=wide if qkv_stride is None else int(qkv_stride),
+        out_stride=nq * hd if out_stride is None else int(out_stride), R=R, nq=nq, nkv=nkv, hd=hd, prefix_len=P,
+        max_len=max_len, rope_len=rope.shape[0], cache_dtype=code, qkv_dtype=_dtype_code(qkv_dtype),
+        out_dtype=_dtype_code(out_dtype), eps=float(eps), scale=float(scale or 0.0))
+    p.addr = ctypes.addressof(p.desc)
+    p.device, p.index, p.hd = dev, dev.index, hd
+    p.qkv_shape, p.out_shape = torch.Size((R, wide)), torch.Size((R, nq * hd))
+    p.qkv_dtype, p.out_dtype = qkv_dtype, out_dtype
+    p.qkv_stride, p.out_stride = (p.desc.qkv_stride, 1), (p.desc.out_stride, 1)
+    p.workspace = workspace
+    p.keep = (K, V, Kp, Vp, mass, rope, pos, rows)
+    return p
+
+
+def decode_attention_shared(plan: SharedDecodePlan, qkv: torch.Tensor, qn: torch.Tensor, kn: torch.Tensor,
+                            out: torch.Tensor | None = None) -> torch.Tensor:
+    """One decode step of one layer for all requests of `plan`: appends each live request's k and v to its own
+    cache (row rows[r]), attends over the shared prefix and its own rows, adds the own rows' attention
+    weights to the plan's mass. qkv (R, (nq + 2*nkv)*hd); qn, kn float32 (hd,); returns out (R, nq*hd), rows
+    of idle slots left as they were. The prefix is read once for all requests."""
+    if out is None:
+        _need(plan.out_stride[0] == plan.out_shape[1], "a plan with an out_stride needs out=")
+        out = torch.empty(plan.out_shape, device=plan.device, dtype=plan.out_dtype)
+    dev, f32, hd = plan.device, torch.float32, plan.hd
+    one = plan.qkv_shape[0] == 1
+    if not (qkv.dtype is plan.qkv_dtype and qkv.device == dev and qkv.shape == plan.qkv_shape
+            and (qkv.stride() == plan.qkv_stride or one and qkv.stride(1) == 1)):
+        raise ValueError(f"qkv must be {tuple(plan.qkv_shape)} {plan.qkv_dtype} on {dev}, strides {plan.qkv_stride}")
+    if not (out.dtype is plan.out_dtype and out.device == dev and out.shape == plan.out_shape
+            and (out.stride() == plan.out_stride or one and out.stride(1) == 1)):
+        raise ValueError(f"out must be {tuple(plan.out_shape)} {plan.out_dtype} on {dev}, strides {plan.out_stride}")
+    if not (qn.dtype is f32 and kn.dtype is f32 and qn.numel() == hd and kn.numel() == hd and qn.is_contiguous()
+            and kn.is_contiguous() and qn.device == dev and kn.device == dev):
+        raise ValueError(f"qn and kn must be contiguous float32 ({hd},) on {dev}")
+    if torch.cuda.current_device() != plan.index:
+        with torch.cuda.device(plan.index):
+            return decode_attention_shared(plan, qkv, qn, kn, out)
+    if _NVTX:
+        with _nvtx("sk_decode_attention_shared"):
+            rc = lib().sk_decode_attention_shared(plan.addr, qkv.data_ptr(), qn.data_ptr(), kn.data_ptr(),
+                                                  out.data_ptr(), _raw_stream(plan.index))
+    else:
+        rc = lib().sk_decode_attention_shared(plan.addr, qkv.data_ptr(), qn.data_ptr(), kn.data_ptr(), out.data_ptr(),
+                                              _raw_stream(plan.index))
+    if rc:
+        check(rc, "sk_decode_attention_shared")
+    return out
+
+
+class CacheEvictPlan:
+    """The checked arguments of cache_evict (see cache_evict_plan). Holds the tensors it points into."""
+
+    __slots__ = ("desc", "addr", "index", "keep", "out", "workspace")
+
+
+def cache_evict_plan(K: torch.Tensor, V: torch.Tensor, mass: torch.Tensor, rows: torch.Tensor, keep: int,
+                     first: int = 0, recent: int = 0,
+                     out: tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor] | None = None,
+                     workspace: torch.Tensor | None = None) -> CacheEvictPlan:
+    """What cache_evict works on, checked once.
+
+    K, V: caches (N, R, nkv, max_len, hd) or (R, nkv, max_len, hd), bf16 or fp32, rows contiguous, any strides
+    else; mass float32, the same without hd; rows int64 (R,): rows held, negative for an idle slot. Caches of
+    more than `keep` rows keep their `first` first, their `recent` last and those with the greatest mass of
+    the rest, in their order. out: (K, V, mass, rows) to write to (their max_len at least keep; rows may be
+    `rows` itself), None: in place, `rows` too. workspace: a uint8 buffer of the size the plan needs (None:
+    made here; plan.workspace), which calls that may run at the same time must not share."""
+    _need(K.is_cuda, "K must be a CUDA tensor")
+    dev, dt = K.device, K.dtype
+    code = _dtype_code(dt)
+    held = (K, V, mass, rows) if out is None else (K, V, mass, rows, *out)
+    five = lambda t: t if t.dim() == 5 else t.unsqueeze(0)  # noqa: E731
+    four = lambda t: t if t.dim() == 4 else t.unsqueeze(0)  # noqa: E731
+
+    def checked(name, k, v, m, r):
+        _need(k.dim() in (4, 5) and k.shape == v.shape and k.stride() == v.stride(),
+              f"{name}K and V must be (N, R, nkv, max_len, hd) or (R, nkv, max_len, hd), laid out alike")
+        _need(m.shape == k.shape[:-1], f"{name}mass must be {tuple(k.shape[:-1])}")
+        k, v, m = five(k), five(v), four(m)
+        _need(k.stride(4) == 1 and (m.stride(3) == 1 or m.shape[3] == 1), f"{name}rows must be contiguous")
+        _need(r.shape == (k.shape[1],) and r.is_contiguous(), f"{name}rows must be contiguous ({k.shape[1]},)")
+        for n, t, want in (("K", k, dt), ("V", v, dt), ("mass", m, torch.float32), ("rows", r, torch.int64)):
+            _need(t.device == dev and t.dtype == want, f"{name}{n} must be {want} on {dev}")
+        return k, v, m, r
+
+    def strides(t, n):  # of dimensions of one element any stride will do: a positive, aligned one
+        return [s if e > 1 else t.shape[-1] for s, e in zip(t.stride()[:n], t.shape[:n])]
+
+    k, v, m, r = checked("", K, V, mass, rows)
+    if out is None:
+        ko, vo, mo, ro = k, v, m, r
+    else:
+        ko, vo, mo, ro = checked("out ", *out)
+        _need(ko.shape[:3] == k.shape[:3] and ko.shape[4] == k.shape[4], "out must hold the same layers, requests and heads")
+    N, R, nkv, max_len, hd = k.shape
+    p = CacheEvictPlan()
+    ll = lambda xs: (ctypes.c_longlong * len(xs))(*xs)  # noqa: E731
+    p.desc = _lib.SkCacheEvict(
+        K=_ptr(k), V=_ptr(v), mass=_ptr(m), kv_stride=ll(strides(k, 4)), mass_stride=ll(strides(m, 3)), K_out=_ptr(ko),
+        V_out=_ptr(vo), mass_out=_ptr(mo), kv_out_stride=ll(strides(ko, 4)), mass_out_stride=ll(strides(mo, 3)),
+        rows=_ptr(r), rows_out=_ptr(ro), N=N, R=R, nkv=nkv, hd=hd, max_len=max_len, max_len_out=ko.shape[3],
+        keep=int(keep), first=int(first), recent=int(recent), cache_dtype=code)
+    n = int(lib().sk_cache_evict_workspace_bytes(ctypes.byref(p.desc)))
+    _need(n > 0, f"unsupported sizes or budget: caches {tuple(k.shape)} to {ko.shape[3]} rows, keep={keep} first={first} "
+                 f"recent={recent}")
+    if workspace is None:
+        workspace = torch.empty(n, dtype=torch.uint8, device=dev)
+    _need(workspace.device == dev and workspace.is_contiguous(), f"workspace must be contiguous on {dev}")
+    p.desc.workspace, p.desc.ws_bytes = _ptr(workspace), workspace.numel() * workspace.element_size()
+    p.addr, p.index, p.workspace = ctypes.addressof(p.desc), dev.index, workspace
+    p.out = (K, V, mass, rows) if out is None else out
+    p.keep = held
+    return p
+
+
+def cache_evict(plan: CacheEvictPlan) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Evicts the caches of `plan` down to its budget; returns the (K, V, mass, rows) written to."""
+    if torch.cuda.current_device() != plan.index:
+        with torch.cuda.device(plan.index):
+            return cache_evict(plan)
+    with _nvtx("sk_cache_evict"):
+        rc = lib().sk_cache_evict(plan.addr, _raw_stream(plan.index))
+    if rc:
+        check(rc, "sk_cache_evict")
+    return plan.out
+
+
 def version() -> int:
     return int(lib().sk_version())
 
 
 __all__ = ["dit_qkv_prologue", "dit_attention", "sdpa", "decode_attention", "decode_workspace",
            "decode_attention_block", "decode_block_workspace", "decode_attention_grouped", "decode_requests",
-           "decode_workspace_bytes", "device_error", "version", "_lib"]
+           "decode_workspace_bytes", "shared_decode_plan", "shared_decode_workspace", "SharedDecodePlan",
+           "decode_attention_shared", "cache_evict_plan", "CacheEvictPlan", "cache_evict", "device_error", "version",
+           "_lib"]
