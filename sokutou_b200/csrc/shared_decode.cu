@@ -40,10 +40,6 @@ __device__ __forceinline__ float warp_max(float v) {
   for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
-__device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void griddep_launch_dependents() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
 // 16 bytes to shared memory; `keep` false writes zeros (and reads nothing).
 __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool keep) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(keep ? 16 : 0)
@@ -65,7 +61,7 @@ struct SimtSmem {
   static constexpr int OFF_P = OFF_V + KT * PITCH * (int)sizeof(T);
   static constexpr int OFF_ST = OFF_P + RT * KT * 4;      // m, l, alpha per row
   static constexpr int OFF_CUM = OFF_ST + 3 * RT * 4;
-  static __host__ __device__ int bytes(int R) { return OFF_CUM + (R + 1) * 4; }
+  static __host__ __device__ int bytes(int R) { return OFF_CUM + Lens::bytes(R); }
 };
 
 template <typename T, int HD>
@@ -80,25 +76,22 @@ __global__ void __launch_bounds__(kSimtThreads) tiles_simt_kernel(const Params p
   float* m_s = reinterpret_cast<float*>(smem + S::OFF_ST);
   float* l_s = m_s + RT;
   float* a_s = l_s + RT;
-  int* cum = reinterpret_cast<int*>(smem + S::OFF_CUM);
+  const Lens ls(smem + S::OFF_CUM, p.R);
   __shared__ int any_s;
   const int t = threadIdx.x, lane = t & 31, w = t >> 5, c = blockIdx.x;
 
   griddep_wait();
   griddep_launch_dependents();
   if (w == 0) {
-    const bool any = scan_tiles<KT>(p, cum, c == 0);
+    const bool any = scan_tiles<KT>(p, ls, c == 0);
     if (lane == 0) any_s = any;
   }
   __syncthreads();
   if (c == 0)
-    for (int r = t; r <= p.R; r += kSimtThreads) p.cum[r] = cum[r];
-  const Tiles tl = tiles_of<CutSimt>(p, cum[p.R], any_s);
-  const long long end = share_begin(tl, c + 1);
-
-  for (long long tile = share_begin(tl, c); tile < end;) {
-    const Segment sg = segment_at<CutSimt>(p, tl, cum, tile, end);
-    tile += sg.t1 - sg.t0;
+    for (int r = t; r <= p.R; r += kSimtThreads) p.cum[r] = ls.cum[r];
+  const Tiles tl = tiles_of<CutSimt>(p, ls.cum[p.R], any_s);
+  Segments sg;
+  for (bool more = sg.first(p, tl, ls, c); more; more = sg.next(p, tl, ls)) {
     const int row0 = sg.prefix ? sg.r * RT : 0;
     const int n_rows = sg.prefix ? min(RT, p.R * p.g - row0) : p.g;
     const T* Kb = sg.prefix ? reinterpret_cast<const T*>(p.Kp) + sg.kvh * p.prefix_head_stride
@@ -110,10 +103,9 @@ __global__ void __launch_bounds__(kSimtThreads) tiles_simt_kernel(const Params p
     for (int i = w; i < n_rows; i += kSimtThreads / 32) {
       const int r = sg.prefix ? (row0 + i) / p.g : sg.r, h = sg.prefix ? (row0 + i) % p.g : i;
       float x[E] = {};
-      bool bad = false;
-      if (own_rows(p, r, &bad) >= 0) {
+      if (ls.len[r] >= 0) {
         load_row<HD>(p.qkv, r * p.qkv_stride + (long long)(sg.kvh * p.g + h) * HD, p.qkv_bf16, x);
-        norm_rotate<HD>(x, p.qn, p.rope + p.pos[r] * HD, p.eps);
+        norm_rotate<HD>(x, p.qn, p.rope, ls.pos[r], p.eps);
 #pragma unroll
         for (int e = 0; e < E; ++e) x[e] *= p.q_scale;
       }
@@ -218,7 +210,7 @@ constexpr int kJoinThreads = 256, kMassChunk = 1024;
 
 template <class Cut, typename T, int HD>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
-  constexpr int E = HD / 32, OQ = Cut::OQ, RT = Cut::RT;
+  constexpr int E = HD / 32, RT = Cut::RT;
   __shared__ float snew_s[kMaxGroup], M_s[kMaxGroup], iL_s[kMaxGroup];
   __shared__ __align__(16) float red_s[kJoinThreads / 32][HD];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
@@ -230,7 +222,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
   if (n < 0 || (blockIdx.y > 0 && (int)blockIdx.y * kMassChunk >= n)) return;
 
   const int per = max(1, (kJoinThreads / 32) / p.g), h = w / per, sub = w % per;  // warps per head
-  const float* turn = p.rope + p.pos[r] * HD;
+  const int pos = (int)p.pos[r];
   float v[E] = {};
   float acc[E] = {};
   float w_new = 0.f;
@@ -240,8 +232,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
     load_row<HD>(p.qkv, base + (long long)(kvh * p.g + h) * HD, p.qkv_bf16, q);
     load_row<HD>(p.qkv, base + (long long)(p.nq + kvh) * HD, p.qkv_bf16, k);
     load_row<HD>(p.qkv, base + (long long)(p.nq + p.nkv + kvh) * HD, p.qkv_bf16, v);
-    norm_rotate<HD>(q, p.qn, turn, p.eps);
-    norm_rotate<HD>(k, p.kn, turn, p.eps);
+    norm_rotate<HD>(q, p.qn, p.rope, pos, p.eps);
+    norm_rotate<HD>(k, p.kn, p.rope, pos, p.eps);
     float dot = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -261,24 +253,22 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
     // where this head's partials lie
     const Tiles tl = tiles_of<Cut>(p, p.cum[p.R], true);
     const int i = r * p.g + h, rt = i / RT, il = i - rt * RT;
-    const bool split = OQ > 1 && min(RT, p.R * p.g - rt * RT) <= RT / OQ;  // the tile's rows ran once per key quarter
-    const int pq = split ? OQ : 1, ip = kvh * tl.nrt + rt;
+    const int ip = kvh * tl.nrt + rt;
     int pc = 0, np = 0;
     if (tl.tp > 0) {
-      pc = share_of(tl, (long long)ip * tl.tp);
-      np = (share_of(tl, (long long)(ip + 1) * tl.tp - 1) - pc + 1) * pq;
+      pc = share_of(tl, ip * tl.tp);
+      np = share_of(tl, (ip + 1) * tl.tp - 1) - pc + 1;
     }
     const int tr = p.cum[r + 1] - p.cum[r], io = r * p.nkv + kvh;
     int oc = 0, no = 0;
     if (tr > 0) {
-      const long long first = tl.n_prefix + (long long)p.cum[r] * p.nkv + (long long)kvh * tr;
+      const int first = tl.n_prefix + p.cum[r] * p.nkv + kvh * tr;
       oc = share_of(tl, first);
-      no = (share_of(tl, first + tr - 1) - oc + 1) * OQ;
+      no = share_of(tl, first + tr - 1) - oc + 1;
     }
     auto place = [&](int x) -> long long {  // partial row of partial x, own rows counted from np
-      if (x < np) return ((long long)(pc + x / pq) + ip) * RT + il + (x % pq) * (RT / OQ);
-      x -= np;
-      return (((long long)(oc + x / OQ) + io) * OQ + x % OQ) * p.g + h;
+      if (x < np) return (long long)(pc + x + ip) * RT + il;
+      return (long long)(oc + x - np + io) * p.g + h;
     };
     float M = s_new;
     for (int x = lane; x < np + no; x += 32) M = fmaxf(M, __ldcg((x < np ? p.pml : p.oml) + 2 * place(x)));
@@ -353,7 +343,7 @@ static int check_sizes(const SkSharedDecode* d) {
     return SK_ERR_INVALID_ARG;
   if (d->nq % d->nkv != 0 || d->nq / d->nkv > kMaxGroup || d->R > kMaxRequests || d->nkv > 1024)
     return SK_ERR_UNSUPPORTED;
-  if (d->prefix_len > (1 << 30) || d->max_len > (1 << 30)) return SK_ERR_UNSUPPORTED;
+  if (too_many_tiles<CutSimt>(d->R, d->nq / d->nkv, d->nkv, d->prefix_len, d->max_len)) return SK_ERR_UNSUPPORTED;
   return SK_OK;
 }
 
@@ -392,13 +382,25 @@ static int launch_simt(const Params& p, cudaStream_t st) {
   return launch_join<CutSimt, T, HD>(p, st);
 }
 
+template <int HD>
+static int launch_tc(const Params& p, bool p_split, cudaStream_t st) {
+  const int rc = launch_tiles_tc(p, HD, p_split, st);
+  return rc != SK_OK ? rc : launch_join<CutTc, __nv_bfloat16, HD>(p, st);
+}
+
+static WsLayout layout_of(const SkSharedDecode* d) {
+  return d->cache_dtype == SK_BF16
+             ? ws_layout<CutTc>(d->R, d->nq, d->nkv, d->hd, d->prefix_len, d->max_len, d->mass != nullptr)
+             : ws_layout<CutSimt>(d->R, d->nq, d->nkv, d->hd, d->prefix_len, d->max_len, d->mass != nullptr);
+}
+
 }  // namespace shared
 }  // namespace sk
 
 extern "C" size_t sk_decode_shared_workspace_bytes(const SkSharedDecode* d) {
   using namespace sk::shared;
   if (check_sizes(d) != SK_OK) return 0;
-  return (size_t)ws_layout<CutSimt>(d->R, d->nq, d->nkv, d->hd, d->prefix_len, d->max_len, d->mass != nullptr).bytes;
+  return (size_t)layout_of(d).bytes;
 }
 
 extern "C" int sk_decode_attention_shared(const SkSharedDecode* d, const void* qkv, const float* qn, const float* kn,
@@ -430,7 +432,7 @@ extern "C" int sk_decode_attention_shared(const SkSharedDecode* d, const void* q
   if (d->mass && ((reinterpret_cast<uintptr_t>(d->mass) & 3) || (d->R > 1 && d->mass_request_stride < 1) ||
                   (d->nkv > 1 && d->mass_head_stride < 1)))
     return SK_ERR_INVALID_ARG;
-  const WsLayout w = ws_layout<CutSimt>(d->R, d->nq, d->nkv, hd, d->prefix_len, d->max_len, d->mass != nullptr);
+  const WsLayout w = layout_of(d);
   if (!d->workspace || (reinterpret_cast<uintptr_t>(d->workspace) & 255) || d->ws_bytes < (size_t)w.bytes)
     return SK_ERR_WORKSPACE;
   const int dev = sk_check_device();
@@ -459,6 +461,6 @@ extern "C" int sk_decode_attention_shared(const SkSharedDecode* d, const void* q
   if (!p.err) return SK_ERR_CUDA;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (d->cache_dtype == SK_BF16)
-    return hd == 128 ? launch_simt<__nv_bfloat16, 128>(p, st) : launch_simt<__nv_bfloat16, 64>(p, st);
+    return hd == 128 ? launch_tc<128>(p, !o16, st) : launch_tc<64>(p, !o16, st);
   return hd == 128 ? launch_simt<float, 128>(p, st) : launch_simt<float, 64>(p, st);
 }

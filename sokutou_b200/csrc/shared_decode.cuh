@@ -4,7 +4,7 @@
 // Work. The keys of a step are cut into tiles of KT rows: first the prefix, per (key/value head, tile of RT
 // query rows) an item of ceil(P / KT) tiles — query row i = r*g + h of a head, all requests together —, then
 // the own rows, per (request, key/value head) an item of ceil(n / KT) tiles. All tiles in one row, item
-// after item, are split evenly over G = min(grid, N) CTAs (floor(N*c/G) .. floor(N*(c+1)/G)): every CTA
+// after item, are split evenly over the CTAs, one more for the first N mod G: every CTA
 // moves the same number of bytes whatever the lengths are, and an item is cut only where a CTA's share
 // ends. The part of an item that one CTA does is a segment; it leaves one partial (running max, sum,
 // unnormalised output) per query row. Along the row of tiles the pair (CTA, item) never steps back in
@@ -20,6 +20,11 @@ namespace shared {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxRequests = 1024;
 constexpr int kMaxGroup = 8;
+
+__device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void griddep_launch_dependents() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
 
 struct Params {
   const void* Kp;
@@ -44,21 +49,26 @@ struct Params {
   int* cum;            // [R + 1] own tiles of the requests before r, per head (written by CTA 0)
   float* po;           // prefix partials [CTA + item][RT][hd]; ml [..][RT][2]
   float* pml;
-  float* oo;           // own partials [CTA + item][OL][hd]; ml [..][OL][2]
+  float* oo;           // own partials [CTA + item][g][hd]; ml [..][g][2]
   float* oml;
   float* sc;           // log2-domain scores of the own rows [R][nq][sc_stride] (mass only)
   long long sc_stride;
   int* err;
 };
 
-// How one of the two main kernels cuts the work: key rows per tile, query rows per prefix item, CTAs,
-// partial rows per query head that an own segment leaves (one per quarter of a tile's keys where the
-// four warps of the tensor-core kernel each keep their own running maximum).
-template <int KT_, int RT_, int G_, int OQ_>
+// How one of the two main kernels cuts the work: key rows per tile, query rows per prefix item, CTAs.
+template <int KT_, int RT_, int G_>
 struct CutOf {
-  static constexpr int KT = KT_, RT = RT_, G = G_, OQ = OQ_;
+  static constexpr int KT = KT_, RT = RT_, G = G_;
 };
-using CutSimt = CutOf<64, 16, 296, 1>;  // CUDA cores: two CTAs on each of 148 SMs
+using CutSimt = CutOf<64, 16, 296>;   // CUDA cores: two CTAs on each of 148 SMs
+using CutTc = CutOf<128, 128, 148>;   // tensor cores: one CTA on each
+// All tiles of a step at the most (2^31 and above are refused).
+template <class Cut>
+__host__ inline bool too_many_tiles(long long R, long long g, long long nkv, long long P, long long max_len) {
+  const long long tp = (P + Cut::KT - 1) / Cut::KT, to = (max_len + Cut::KT - 1) / Cut::KT;
+  return nkv * (tp * ((R * g + Cut::RT - 1) / Cut::RT) + R * to) > 0x7fffffffLL;
+}
 
 __host__ __device__ inline long long align_up(long long x, long long a) { return (x + a - 1) / a * a; }
 
@@ -79,8 +89,8 @@ __host__ inline WsLayout ws_layout(int R, int nq, int nkv, int hd, int P, int ma
   w.cum = take((long long)(R + 1) * 4);
   w.po = take(slots_p * Cut::RT * hd * 4);
   w.pml = take(slots_p * Cut::RT * 8);
-  w.oo = take(slots_o * Cut::OQ * g * hd * 4);
-  w.oml = take(slots_o * Cut::OQ * g * 8);
+  w.oo = take(slots_o * g * hd * 4);
+  w.oml = take(slots_o * g * 8);
   w.sc_stride = align_up(max_len, 128);
   w.sc = take(mass ? (long long)R * nq * w.sc_stride * 4 : 0);
   w.bytes = at;
@@ -89,9 +99,9 @@ __host__ inline WsLayout ws_layout(int R, int nq, int nkv, int hd, int P, int ma
 
 // Own rows of request r before this step, -1 if the slot is idle (or out of range: *bad).
 __device__ __forceinline__ int own_rows(const Params& p, int r, bool* bad) {
-  const long long pos = p.pos[r];
+  const long long pos = p.pos[r], own = p.rows ? p.rows[r] : pos - p.P;  // both loads at once
   if (pos < 0) return -1;
-  const long long n = p.rows ? p.rows[r] : pos - p.P;
+  const long long n = own;
   if (pos >= p.rope_len || n < 0 || n >= p.max_len) {
     *bad = true;
     return -1;
@@ -99,11 +109,17 @@ __device__ __forceinline__ int own_rows(const Params& p, int r, bool* bad) {
   return (int)n;
 }
 
-// One warp: cum_s[r] = own tiles per head of the requests before r (cum_s[R]: of all), and whether any
-// request is live; records positions out of range. Sixteen requests' lengths are in flight per lane pair
-// of loads, so a server of 64 pays for one trip to L2.
+// One warp: for every request its own tiles per head before it (cum[R]: of all), its own rows (-1: idle) and
+// its position; whether any is live; records positions out of range.
+struct Lens {  // shared memory, kMaxRequests-bounded
+  int* cum;    // [R + 1]
+  int* len;    // [R]
+  int* pos;    // [R]
+  static __host__ __device__ int bytes(int R) { return (3 * R + 1) * 4; }
+  __device__ __forceinline__ Lens(void* at, int R) : cum((int*)at), len(cum + R + 1), pos(len + R) {}
+};
 template <int KT>
-__device__ __forceinline__ bool scan_tiles(const Params& p, int* cum_s, bool report) {
+__device__ __forceinline__ bool scan_tiles(const Params& p, const Lens& s, bool report) {
   const int lane = threadIdx.x & 31;
   int base = 0;
   bool any = false, bad = false;
@@ -118,81 +134,120 @@ __device__ __forceinline__ bool scan_tiles(const Params& p, int* cum_s, bool rep
       const int y = __shfl_up_sync(0xffffffffu, x, o);
       if (lane >= o) x += y;
     }
-    if (r < p.R) cum_s[r] = base + x - own;
+    if (r < p.R) {
+      s.cum[r] = base + x - own;
+      s.len[r] = n;
+      s.pos[r] = n >= 0 ? (int)p.pos[r] : 0;
+    }
     base += __shfl_sync(0xffffffffu, x, 31);
   }
-  if (lane == 0) cum_s[p.R] = base;
+  if (lane == 0) s.cum[p.R] = base;
   if (report && bad) set_dev_error(p.err, SK_DEVERR_POS_RANGE);
   return __any_sync(0xffffffffu, any);
 }
 
-// The row of tiles of one step.
+// The row of tiles of one step (the host refuses sizes with 2^31 tiles).
 struct Tiles {
-  int tp;             // tiles of a prefix item
-  int nrt;            // prefix items per head
-  long long n_prefix; // tiles of all prefix items
-  long long n;        // all tiles
-  int G;              // CTAs with work: min(grid, n), so that none between two of an item's is without a part
+  int tp;          // tiles of a prefix item
+  int nrt;         // prefix items per head
+  int n_prefix;    // tiles of all prefix items
+  int n;           // all tiles
+  int each, more;  // a share is `each` tiles, one more for the first `more` CTAs
 };
 template <class Cut>
 __device__ __forceinline__ Tiles tiles_of(const Params& p, int own_tiles, bool any) {
   Tiles t;
-  t.tp = any ? (p.P + Cut::KT - 1) / Cut::KT : 0;
-  t.nrt = (p.R * p.g + Cut::RT - 1) / Cut::RT;
-  t.n_prefix = (long long)t.tp * t.nrt * p.nkv;
-  t.n = t.n_prefix + (long long)own_tiles * p.nkv;
-  t.G = (int)min((long long)Cut::G, t.n);
+  t.tp = any ? (int)((uint32_t)(p.P + Cut::KT - 1) / Cut::KT) : 0;
+  t.nrt = (int)((uint32_t)(p.R * p.g + Cut::RT - 1) / Cut::RT);
+  t.n_prefix = t.tp * t.nrt * p.nkv;
+  t.n = t.n_prefix + own_tiles * p.nkv;
+  t.each = (int)((uint32_t)t.n / Cut::G);
+  t.more = t.n - t.each * Cut::G;
   return t;
 }
-__device__ __forceinline__ long long share_begin(const Tiles& t, int c) { return c < t.G ? t.n * c / t.G : t.n; }
-__device__ __forceinline__ int share_of(const Tiles& t, long long tile) {  // the CTA whose share holds `tile`
-  return (int)(((tile + 1) * t.G - 1) / t.n);
+__device__ __forceinline__ int share_begin(const Tiles& t, int c) { return c * t.each + min(c, t.more); }
+__device__ __forceinline__ int share_of(const Tiles& t, int tile) {  // the CTA whose share holds `tile`
+  const uint32_t cut = (uint32_t)t.more * (t.each + 1);
+  return (int)((uint32_t)tile < cut ? (uint32_t)tile / (t.each + 1) : t.more + ((uint32_t)tile - cut) / t.each);
 }
 
-// The part of one item that a CTA does.
-struct Segment {
+// The segments of a CTA's share, one after another.
+struct Segments {
   bool prefix;
-  int item;     // prefix: kvh * nrt + rt; own: r * nkv + kvh
-  int kvh, r;   // r: request (own), or the tile of query rows (prefix)
-  int t0, t1;   // tiles of the item
-  int n_keys;   // rows of the item (prefix: P; own: n)
+  int item;        // prefix: kvh * nrt + rt; own: r * nkv + kvh
+  int kvh, r;      // r: request (own), or the tile of query rows (prefix)
+  int t0, t1;      // tiles of the item
+  int n_keys;      // rows of the item (prefix: P; own: n)
+  int left;        // tiles of the share after this segment
+
+  // The first segment of CTA c's share; false: the share is empty.
+  __device__ __forceinline__ bool first(const Params& p, const Tiles& t, const Lens& s, int c) {
+    const int tile = share_begin(t, c);
+    left = share_begin(t, c + 1) - tile;
+    if (left <= 0) return false;
+    if (tile < t.n_prefix) {
+      prefix = true;
+      item = (int)((uint32_t)tile / t.tp);
+      kvh = (int)((uint32_t)item / t.nrt);
+      r = item - kvh * t.nrt;
+      t0 = tile - item * t.tp;
+      take(t.tp, p.P);
+      return true;
+    }
+    const int o = tile - t.n_prefix;
+    int lo = 0, hi = p.R;  // the last r with cum[r] * nkv <= o: it has tiles
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (s.cum[mid] * p.nkv <= o)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    const int tr = s.cum[lo + 1] - s.cum[lo];
+    const int in_r = o - s.cum[lo] * p.nkv;
+    prefix = false;
+    r = lo;
+    kvh = (int)((uint32_t)in_r / tr);
+    item = lo * p.nkv + kvh;
+    t0 = in_r - kvh * tr;
+    take(tr, s.len[lo]);
+    return true;
+  }
+  // Steps on; false after the last. Items follow one another without gaps, so no division is needed.
+  __device__ __forceinline__ bool next(const Params& p, const Tiles& t, const Lens& s) {
+    if (left <= 0) return false;
+    t0 = 0;
+    if (prefix) {
+      if (++r == t.nrt) {
+        r = 0;
+        ++kvh;
+      }
+      ++item;
+      if (kvh < p.nkv) {
+        take(t.tp, p.P);
+        return true;
+      }
+      prefix = false;
+      r = -1;
+      kvh = p.nkv - 1;
+    }
+    if (++kvh == p.nkv) {
+      kvh = 0;
+      do ++r;
+      while (s.len[r] <= 0);  // a request with tiles follows, as the share goes on
+    }
+    item = r * p.nkv + kvh;
+    take(s.cum[r + 1] - s.cum[r], s.len[r]);
+    return true;
+  }
+
+ private:
+  __device__ __forceinline__ void take(int tiles, int keys) {
+    n_keys = keys;
+    t1 = min(tiles, t0 + left);
+    left -= t1 - t0;
+  }
 };
-// The segment that starts at `tile`, ending at `end` at the latest. cum: the scan of scan_tiles.
-template <class Cut>
-__device__ __forceinline__ Segment segment_at(const Params& p, const Tiles& t, const int* cum, long long tile,
-                                              long long end) {
-  Segment s;
-  if (tile < t.n_prefix) {
-    s.prefix = true;
-    s.item = (int)(tile / t.tp);
-    s.kvh = s.item / t.nrt;
-    s.r = s.item - s.kvh * t.nrt;
-    s.t0 = (int)(tile - (long long)s.item * t.tp);
-    s.t1 = (int)min((long long)t.tp, s.t0 + (end - tile));
-    s.n_keys = p.P;
-    return s;
-  }
-  const long long o = tile - t.n_prefix;
-  int lo = 0, hi = p.R;  // the last r with cum[r] * nkv <= o (and tiles of its own)
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if ((long long)cum[mid] * p.nkv <= o)
-      lo = mid;
-    else
-      hi = mid;
-  }
-  const int tr = cum[lo + 1] - cum[lo];
-  const int in_r = (int)(o - (long long)cum[lo] * p.nkv);
-  s.prefix = false;
-  s.r = lo;
-  s.kvh = in_r / tr;
-  s.item = lo * p.nkv + s.kvh;
-  s.t0 = in_r - s.kvh * tr;
-  s.t1 = (int)min((long long)tr, s.t0 + (end - tile));
-  bool bad = false;
-  s.n_keys = own_rows(p, lo, &bad);
-  return s;
-}
 
 // E consecutive floats, E 2 or 4, aligned to their size.
 template <int E>
@@ -240,29 +295,51 @@ __device__ __forceinline__ void load_row(const void* base, long long at, int is_
     load_vec<E>(reinterpret_cast<const float*>(base) + at + lane * E, x);
   }
 }
-// RMS norm (x w) and rotation of a head row in fp32, the reference's order of operations
-// (qwen3/kernels.py:354-380); `turn` = the rope table's row of the position.
-template <int HD>
-__device__ __forceinline__ void norm_rotate(float (&x)[HD / 32], const float* w, const float* turn, float eps) {
+// RMS norm (x w) and rotation of B head rows in fp32, the reference's order of operations
+// (qwen3/kernels.py:354-380); row b turns by the table's row pos[r[b]]. Every load goes out before the first
+// sum, and the rows' shuffles interleave.
+template <int HD, int B>
+__device__ __forceinline__ void norm_rotate_rows(float (&x)[B][HD / 32], const int (&r)[B], const int* pos,
+                                                 const float* w, const float* rope, float eps) {
   constexpr int E = HD / 32;
   const int lane = threadIdx.x & 31;
-  float ss = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) ss += x[e] * x[e];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  const float inv = rsqrtf(ss / HD + eps);
-  float wv[E], c[E], s[E];
+  float wv[E], c[B][E], s[B][E], ss[B];
   load_vec<E>(w + lane * E, wv);
-  load_vec<E>(turn + (lane & 15) * E, c);
-  load_vec<E>(turn + HD / 2 + (lane & 15) * E, s);
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const float y = x[e] * inv * wv[e];
-    const float other = __shfl_xor_sync(0xffffffffu, y, 16);
-    x[e] = y * c[e] + (lane < 16 ? -other : other) * s[e];
+  for (int b = 0; b < B; ++b) {
+    const float* turn = rope + (long long)pos[r[b]] * HD + (lane & 15) * E;
+    load_vec<E>(turn, c[b]);
+    load_vec<E>(turn + HD / 2, s[b]);
+  }
+#pragma unroll
+  for (int b = 0; b < B; ++b) {
+    ss[b] = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) ss[b] += x[b][e] * x[b][e];
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int b = 0; b < B; ++b) ss[b] += __shfl_xor_sync(0xffffffffu, ss[b], o);
+#pragma unroll
+  for (int b = 0; b < B; ++b) {
+    const float inv = rsqrtf(ss[b] / HD + eps);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float y = x[b][e] * inv * wv[e];
+      const float other = __shfl_xor_sync(0xffffffffu, y, 16);
+      x[b][e] = y * c[b][e] + (lane < 16 ? -other : other) * s[b][e];
+    }
   }
 }
+template <int HD>
+__device__ __forceinline__ void norm_rotate(float (&x)[HD / 32], const float* w, const float* rope, int pos, float eps) {
+  const int zero[1] = {0};
+  norm_rotate_rows<HD, 1>(reinterpret_cast<float (&)[1][HD / 32]>(x), zero, &pos, w, rope, eps);
+}
+
+// shared_decode_tc.cu: the key tiles on the tensor cores (bf16 caches); p_split: the weights in two bf16 terms.
+int launch_tiles_tc(const Params& p, int hd, bool p_split, cudaStream_t st);
 
 }  // namespace shared
 }  // namespace sk
