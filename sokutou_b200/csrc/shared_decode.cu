@@ -87,8 +87,6 @@ __global__ void __launch_bounds__(kSimtThreads) tiles_simt_kernel(const Params p
     if (lane == 0) any_s = any;
   }
   __syncthreads();
-  if (c == 0)
-    for (int r = t; r <= p.R; r += kSimtThreads) p.cum[r] = ls.cum[r];
   const Tiles tl = tiles_of<CutSimt>(p, ls.cum[p.R], any_s);
   Segments sg;
   for (bool more = sg.first(p, tl, ls, c); more; more = sg.next(p, tl, ls)) {
@@ -205,29 +203,52 @@ __global__ void __launch_bounds__(kSimtThreads) tiles_simt_kernel(const Params p
 // n, attended as the cache holds them), the partials of the prefix and of the own rows, out, and, a chunk
 // of kMassChunk rows per CTA of grid row y, the weights 2^(s - M) / L added to the mass. An item's
 // partials lie in the slots of the CTAs from the one that holds its first tile to the one that holds its
-// last. The 8 warps are shared out over the heads of the group; a warp reads whole output rows.
-constexpr int kJoinThreads = 256, kMassChunk = 1024;
+// last. The 8 warps are shared out over the heads of the group; a warp reads whole output rows, each with
+// its (max, sum) at once, and keeps a running maximum of its own, so there is one trip to memory for all.
+// What needs no partial — where they lie, the new token — comes before the wait for the key tiles: launched
+// early (programmatic dependent launch, next to the tiles' CTA on each SM) it is done by then. By that time
+// the tiles' kernel has waited for everything before it, so this one may read the activations too.
+constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32, kMassChunk = 1024;
 
 template <class Cut, typename T, int HD>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
-  constexpr int E = HD / 32, RT = Cut::RT;
+  constexpr int E = HD / 32, RT = Cut::RT, KT = Cut::KT;
   __shared__ float snew_s[kMaxGroup], M_s[kMaxGroup], iL_s[kMaxGroup];
-  __shared__ __align__(16) float red_s[kJoinThreads / 32][HD];
+  __shared__ __align__(16) float red_s[kJoinWarps][HD];
+  __shared__ float2 ml_s[kJoinWarps];
+  __shared__ int before_s[kJoinWarps], all_s[kJoinWarps];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int r = blockIdx.x / p.nkv, kvh = blockIdx.x % p.nkv;
-  griddep_wait();  // every thread, before any exit: the kernel after this one relies on it
   griddep_launch_dependents();
   bool bad = false;
   const int n = own_rows(p, r, &bad);
-  if (n < 0 || (blockIdx.y > 0 && (int)blockIdx.y * kMassChunk >= n)) return;
-
-  const int per = max(1, (kJoinThreads / 32) / p.g), h = w / per, sub = w % per;  // warps per head
-  const int pos = (int)p.pos[r];
-  float v[E] = {};
+  if (n < 0 || (blockIdx.y > 0 && (int)blockIdx.y * kMassChunk >= n)) {
+    griddep_wait();  // every thread, before any exit: the kernel after this one relies on it
+    return;
+  }
+  {  // own tiles of the requests before this one, and of all
+    int before = 0, all = 0;
+    for (int x = threadIdx.x; x < p.R; x += kJoinThreads) {
+      const int k = own_rows(p, x, &bad), tiles = k > 0 ? (k + KT - 1) / KT : 0;
+      all += tiles;
+      if (x < r) before += tiles;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      before += __shfl_xor_sync(0xffffffffu, before, o);
+      all += __shfl_xor_sync(0xffffffffu, all, o);
+    }
+    if (lane == 0) {
+      before_s[w] = before;
+      all_s[w] = all;
+    }
+  }
+  const int per = max(1, kJoinWarps / p.g), h = w / per, sub = w % per;  // warps per head
   float acc[E] = {};
-  float w_new = 0.f;
+  float m_run = -INFINITY, l_run = 0.f;
   if (h < p.g) {
-    float q[E], k[E];
+    const int pos = (int)p.pos[r];
+    float q[E], k[E], v[E];
     const long long base = r * p.qkv_stride;
     load_row<HD>(p.qkv, base + (long long)(kvh * p.g + h) * HD, p.qkv_bf16, q);
     load_row<HD>(p.qkv, base + (long long)(p.nq + kvh) * HD, p.qkv_bf16, k);
@@ -242,6 +263,13 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
       dot += q[e] * p.q_scale * k[e];
     }
     const float s_new = warp_sum(dot);
+    if (sub == 0) {  // the new token is this warp's first partial
+      m_run = s_new;
+      l_run = 1.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = v[e];
+      if (lane == 0) snew_s[h] = s_new;
+    }
     if (w == 0 && blockIdx.y == 0) {
       const long long at = r * p.request_stride + kvh * p.head_stride + n * p.row_stride + lane * E;
 #pragma unroll
@@ -250,75 +278,104 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
         reinterpret_cast<T*>(p.Vc)[at + e] = Elem<T>::st(v[e]);
       }
     }
-    // where this head's partials lie
-    const Tiles tl = tiles_of<Cut>(p, p.cum[p.R], true);
-    const int i = r * p.g + h, rt = i / RT, il = i - rt * RT;
-    const int ip = kvh * tl.nrt + rt;
-    int pc = 0, np = 0;
-    if (tl.tp > 0) {
-      pc = share_of(tl, ip * tl.tp);
-      np = share_of(tl, (ip + 1) * tl.tp - 1) - pc + 1;
-    }
-    const int tr = p.cum[r + 1] - p.cum[r], io = r * p.nkv + kvh;
-    int oc = 0, no = 0;
-    if (tr > 0) {
-      const int first = tl.n_prefix + p.cum[r] * p.nkv + kvh * tr;
-      oc = share_of(tl, first);
-      no = share_of(tl, first + tr - 1) - oc + 1;
-    }
-    auto place = [&](int x) -> long long {  // partial row of partial x, own rows counted from np
-      if (x < np) return (long long)(pc + x + ip) * RT + il;
-      return (long long)(oc + x - np + io) * p.g + h;
-    };
-    float M = s_new;
-    for (int x = lane; x < np + no; x += 32) M = fmaxf(M, __ldcg((x < np ? p.pml : p.oml) + 2 * place(x)));
-    M = warp_max(M);
-    float L = 0.f;
-    for (int x = lane; x < np + no; x += 32) {
-      const float2 ml = __ldcg(reinterpret_cast<const float2*>((x < np ? p.pml : p.oml) + 2 * place(x)));
-      L += ml.y * ex2_approx(ml.x - M);
-    }
-    w_new = ex2_approx(s_new - M);
-    L = warp_sum(L) + w_new;
-    if (sub == 0 && lane == 0) {
-      snew_s[h] = s_new;
-      M_s[h] = M;
-      iL_s[h] = 1.f / L;
-    }
-    if (blockIdx.y == 0) {
-#pragma unroll 4
-      for (int x = sub; x < np + no; x += per) {
-        const long long at = place(x);
-        const float wt = ex2_approx(__ldcg((x < np ? p.pml : p.oml) + 2 * at) - M);
-        float o[E];
-        load_vec<E>((x < np ? p.po : p.oo) + at * HD + lane * E, o);
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] += wt * o[e];
-      }
-      store_vec<E>(red_s[w] + lane * E, acc);
-    }
   }
   __syncthreads();
-  if (blockIdx.y == 0 && h < p.g && sub == 0) {
+  int before = 0, all = 0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] += w_new * v[e];
-    for (int x = 1; x < per; ++x) {
+  for (int x = 0; x < kJoinWarps; ++x) {
+    before += before_s[x];
+    all += all_s[x];
+  }
+  const Tiles tl = tiles_of<Cut>(p, all, true);
+  const int i = r * p.g + h, rt = i / RT, il = i - rt * RT;
+  const int ip = kvh * tl.nrt + rt, io = r * p.nkv + kvh, tr = (n + KT - 1) / KT;
+  int pc = 0, np = 0, oc = 0, no = 0;
+  if (tl.tp > 0) {
+    pc = share_of(tl, ip * tl.tp);
+    np = share_of(tl, (ip + 1) * tl.tp - 1) - pc + 1;
+  }
+  if (tr > 0) {
+    const int first = tl.n_prefix + before * p.nkv + kvh * tr;
+    oc = share_of(tl, first);
+    no = share_of(tl, first + tr - 1) - oc + 1;
+  }
+  griddep_wait();
+  if (h < p.g) {
+    constexpr int kAhead = 4;
+    for (int x0 = sub; x0 < np + no; x0 += per * kAhead) {
+      float2 ml[kAhead];
+      float o[kAhead][E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] += red_s[w + x][lane * E + e];
+      for (int b = 0; b < kAhead; ++b) {
+        const int x = x0 + b * per;
+        ml[b] = make_float2(-INFINITY, 0.f);
+        if (x < np + no) {
+          const long long at = x < np ? (long long)(pc + x + ip) * RT + il : (long long)(oc + x - np + io) * p.g + h;
+          ml[b] = __ldcg(reinterpret_cast<const float2*>(x < np ? p.pml : p.oml) + at);
+          if (blockIdx.y == 0) load_vec_cg<E>((x < np ? p.po : p.oo) + at * HD + lane * E, o[b]);
+        }
+      }
+      float m = m_run;
+#pragma unroll
+      for (int b = 0; b < kAhead; ++b) m = fmaxf(m, ml[b].x);
+      const float use = m == -INFINITY ? 0.f : m, a = ex2_approx(m_run - use);
+      l_run *= a;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] *= a;
+#pragma unroll
+      for (int b = 0; b < kAhead; ++b) {
+        if (x0 + b * per < np + no) {
+          const float wt = ex2_approx(ml[b].x - use);
+          l_run += wt * ml[b].y;
+          if (blockIdx.y == 0) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] += wt * o[b][e];
+          }
+        }
+      }
+      m_run = m;
     }
-    const long long at = r * p.out_stride + (long long)(kvh * p.g + h) * HD + lane * E;
+    store_vec<E>(red_s[w] + lane * E, acc);
+    if (lane == 0) ml_s[w] = make_float2(m_run, l_run);
+  }
+  __syncthreads();
+  if (h < p.g && sub == 0) {
+    float M = m_run;
+    for (int x = 1; x < per; ++x) M = fmaxf(M, ml_s[w + x].x);
+    float L = 0.f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] *= iL_s[h];
-    if (p.out_bf16) {
-      __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(p.out) + at;
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    for (int x = 0; x < per; ++x) {
+      const float a = ex2_approx(ml_s[w + x].x - M);
+      L += a * ml_s[w + x].y;
+      if (blockIdx.y == 0) {
+        float o[E];
+        load_vec<E>(red_s[w + x] + lane * E, o);
 #pragma unroll
-      for (int e = 0; e < E; e += 2)
-        *reinterpret_cast<__nv_bfloat162*>(o + e) = __floats2bfloat162_rn(acc[e], acc[e + 1]);
-    } else {
-      store_vec<E>(reinterpret_cast<float*>(p.out) + at, acc);
+        for (int e = 0; e < E; ++e) acc[e] += a * o[e];
+      }
+    }
+    const float iL = 1.f / L;
+    if (lane == 0) {
+      M_s[h] = M;
+      iL_s[h] = iL;
+    }
+    if (blockIdx.y == 0) {
+      const long long at = r * p.out_stride + (long long)(kvh * p.g + h) * HD + lane * E;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] *= iL;
+      if (p.out_bf16) {
+        __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(p.out) + at;
+#pragma unroll
+        for (int e = 0; e < E; e += 2)
+          *reinterpret_cast<__nv_bfloat162*>(o + e) = __floats2bfloat162_rn(acc[e], acc[e + 1]);
+      } else {
+        store_vec<E>(reinterpret_cast<float*>(p.out) + at, acc);
+      }
     }
   }
   if (!p.mass) return;
+  __syncthreads();
   float* mass = p.mass + r * p.mass_request_stride + kvh * p.mass_head_stride;
   const float* sc = p.sc + ((long long)r * p.nq + kvh * p.g) * p.sc_stride;
   const int j0 = blockIdx.y * kMassChunk, j1 = min(n, j0 + kMassChunk);
@@ -453,7 +510,6 @@ extern "C" int sk_decode_attention_shared(const SkSharedDecode* d, const void* q
   p.eps = d->eps;
   p.q_scale = (d->scale > 0.f ? d->scale : (hd == 128 ? 0.08838834764831845f : 0.125f)) * kLog2e;
   uint8_t* ws = reinterpret_cast<uint8_t*>(d->workspace);
-  p.cum = reinterpret_cast<int*>(ws + w.cum);
   p.po = reinterpret_cast<float*>(ws + w.po), p.pml = reinterpret_cast<float*>(ws + w.pml);
   p.oo = reinterpret_cast<float*>(ws + w.oo), p.oml = reinterpret_cast<float*>(ws + w.oml);
   p.sc = reinterpret_cast<float*>(ws + w.sc), p.sc_stride = w.sc_stride;

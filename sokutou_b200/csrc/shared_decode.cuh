@@ -46,7 +46,6 @@ struct Params {
   int R, nq, nkv, g, P, max_len, rope_len;
   int qkv_bf16, out_bf16;
   float eps, q_scale;  // softmax scale * log2(e): scores come out in the log2 domain
-  int* cum;            // [R + 1] own tiles of the requests before r, per head (written by CTA 0)
   float* po;           // prefix partials [CTA + item][RT][hd]; ml [..][RT][2]
   float* pml;
   float* oo;           // own partials [CTA + item][g][hd]; ml [..][g][2]
@@ -73,7 +72,7 @@ __host__ inline bool too_many_tiles(long long R, long long g, long long nkv, lon
 __host__ __device__ inline long long align_up(long long x, long long a) { return (x + a - 1) / a * a; }
 
 struct WsLayout {
-  long long cum, po, pml, oo, oml, sc, sc_stride, bytes;
+  long long po, pml, oo, oml, sc, sc_stride, bytes;
 };
 template <class Cut>
 __host__ inline WsLayout ws_layout(int R, int nq, int nkv, int hd, int P, int max_len, bool mass) {
@@ -86,7 +85,6 @@ __host__ inline WsLayout ws_layout(int R, int nq, int nkv, int hd, int P, int ma
     at = align_up(at + n, 256);
     return p;
   };
-  w.cum = take((long long)(R + 1) * 4);
   w.po = take(slots_p * Cut::RT * hd * 4);
   w.pml = take(slots_p * Cut::RT * 8);
   w.oo = take(slots_o * g * hd * 4);
@@ -258,6 +256,16 @@ __device__ __forceinline__ void load_vec(const float* p, float (&x)[E]) {
   } else {
     static_assert(E == 2, "2 or 4");
     const float2 v = *reinterpret_cast<const float2*>(p);
+    x[0] = v.x, x[1] = v.y;
+  }
+}
+template <int E>
+__device__ __forceinline__ void load_vec_cg(const float* p, float (&x)[E]) {  // through L2 only
+  if constexpr (E == 4) {
+    const float4 v = __ldcg(reinterpret_cast<const float4*>(p));
+    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+  } else {
+    const float2 v = __ldcg(reinterpret_cast<const float2*>(p));
     x[0] = v.x, x[1] = v.y;
   }
 }

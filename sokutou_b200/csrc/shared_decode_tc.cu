@@ -32,8 +32,9 @@ namespace shared {
 
 constexpr int kThreadsTc = 384;
 constexpr int kWarpQo = 4, kWarpProducer = 8, kWarpS = 9, kWarpPv = 10, kWarpScan = 11;
-// Launched at 168 registers a thread (64512): softmax 232, query/output 168, the others 80: 61440.
-constexpr int kLaunchRegs = 168, kSoftmaxRegs = 232, kQoRegs = 168, kControlRegs = 80;
+// Launched at 128 registers a thread (49152, which leaves room on the SM for a CTA of the joining kernel, 16384):
+// softmax 168, query/output 128, the others 88.
+constexpr int kLaunchRegs = 128, kSoftmaxRegs = 168, kQoRegs = 128, kControlRegs = 88;
 static_assert(128 * (kSoftmaxRegs + kQoRegs + kControlRegs) <= kThreadsTc * kLaunchRegs, "register split over budget");
 constexpr float kRescale = 8.0f;  // O is rescaled when the running max grows by more than 2^8; exact either way
 
@@ -67,11 +68,14 @@ struct SmemTc {
   static constexpr int OFF_V = OFF_Q + Q_AREA;
   static constexpr int OFF_K = OFF_V + NSV * KV_BYTES;
   static constexpr int OFF_ML = OFF_K + NSK * KV_BYTES;  // [2] n > 32: [128] (max, sum); else sums [4][32], max [32]
-  static constexpr int OFF_MX = OFF_ML + 2 * 128 * 8;    // [4][32] maxima of the warps
-  static constexpr int OFF_BAR = OFF_MX + 4 * 32 * 4;
+  static constexpr int OFF_MX = OFF_ML + 2 * 128 * 8;    // [4][32] maxima of the warps, [32] running, [32] factors
+  static constexpr int OFF_BAR = OFF_MX + 6 * 32 * 4;
   static constexpr int NBAR = 2 * NSK + 2 * NSV + 16;
-  static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;    // tensor-memory base, any live
-  static constexpr int OFF_LENS = OFF_MISC + 16;
+  static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;    // tensor-memory base, whether there is a segment
+  static constexpr int OFF_TILES = OFF_MISC + 16;
+  static constexpr int OFF_SEG = OFF_TILES + 32;
+  static constexpr int OFF_LENS = OFF_SEG + 32;
+  static_assert(sizeof(Tiles) <= 32 && sizeof(Segments) <= 32, "their places in shared memory");
   static __host__ __device__ int bytes(int R) { return OFF_LENS + Lens::bytes(R); }
   static_assert(OFF_LENS + (3 * kMaxRequests + 1) * 4 <= 232448, "shared memory over the 227 KB per-CTA limit");
 };
@@ -140,15 +144,24 @@ __device__ __forceinline__ bool any_of_128(bool x) {
       : "memory");
   return y != 0;
 }
-__device__ __forceinline__ float warp_max_f32(float x) {
-  float y;
-  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float warp_sum_f32(float v) {
+// Sum or maximum over the warp of each of H values per lane (H a power of two up to 32), by halves: lane l
+// returns that of value l * H / 32.
+template <int H, class Op>
+__device__ __forceinline__ float warp_reduce(float (&x)[H], Op op) {
+  const int lane = threadIdx.x & 31;
+  int off = 16;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+  for (int m = H; m > 1; m >>= 1, off >>= 1) {
+    const bool upper = lane & off;
+#pragma unroll
+    for (int i = 0; i < m / 2; ++i) {
+      const float send = upper ? x[i] : x[i + m / 2], keep = upper ? x[i + m / 2] : x[i];
+      x[i] = op(keep, __shfl_xor_sync(0xffffffffu, send, off));
+    }
+  }
+#pragma unroll
+  for (; off > 0; off >>= 1) x[0] = op(x[0], __shfl_xor_sync(0xffffffffu, x[0], off));
+  return x[0];
 }
 
 // Query rows of a segment, and the columns' half width of its transposed form: 8 or 32 (0: the other form).
@@ -158,7 +171,7 @@ __device__ __forceinline__ int rows_of(const Params& p, const Segments& s) {
 __device__ __forceinline__ int form_of(int n) { return n <= 8 ? 8 : n <= 32 ? 32 : 0; }
 
 template <int HD, bool P_SPLIT>
-__global__ void __launch_bounds__(kThreadsTc, 1)
+__global__ void __maxnreg__(kLaunchRegs)
     tiles_tc_kernel(const __grid_constant__ CUtensorMap tmKp, const __grid_constant__ CUtensorMap tmVp,
                     const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                     const __grid_constant__ TcArgs args) {
@@ -214,17 +227,22 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
   griddep_launch_dependents();
   if (warp == kWarpScan) {
     const bool any = scan_tiles<CutTc::KT>(p, ls, c == 0);
-    if (lane == 0) misc[1] = any;
+    __syncwarp();
+    if (lane == 0) {
+      const Tiles tl = tiles_of<CutTc>(p, ls.cum[p.R], any);
+      Segments sg;
+      misc[1] = sg.first(p, tl, ls, c);
+      *reinterpret_cast<Tiles*>(smem + S::OFF_TILES) = tl;
+      *reinterpret_cast<Segments*>(smem + S::OFF_SEG) = sg;
+    }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = misc[0], tS = tmem, tO = tmem + 256;  // S0 S1 | O0 O1, 128 columns each; P over S
-  const Tiles tl = tiles_of<CutTc>(p, ls.cum[p.R], misc[1]);
-  if (c == 0)
-    for (int r = threadIdx.x; r <= p.R; r += kThreadsTc) p.cum[r] = ls.cum[r];
-  Segments sg;
-  bool more = sg.first(p, tl, ls, c);
+  const Tiles tl = *reinterpret_cast<const Tiles*>(smem + S::OFF_TILES);
+  Segments sg = *reinterpret_cast<const Segments*>(smem + S::OFF_SEG);
+  bool more = misc[1];
 
   // The eight working warps keep step with one another (votes, warp-wide loads): a thread whose wait ran out
   // (the error word then says so) goes on to the end without waiting, its results void, rather than leaving.
@@ -330,7 +348,8 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
             for (int term = 0; term < (P_SPLIT ? 2 : 1); ++term)
 #pragma unroll
               for (int kk = 0; kk < 8; ++kk)
-                tc_mma_ts(oc, tS + w * 128 + term * 64 + kk * 8, smem_desc_sw128(vb + kk * 2048, 16384, 1024), id,
+                tc_mma_ts(oc, tS + w * 128 + (kk >> 1) * 32 + (kk & 1) * 8 + term * 16,
+                          smem_desc_sw128(vb + kk * 2048, 16384, 1024), id,
                           t > sg.t0 || term > 0 || kk > 0);
           } else {
 #pragma unroll
@@ -436,7 +455,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
         auto columns = [&](auto half) {  // lane l holds element l of every row
           constexpr int N = decltype(half)::value;
           if (32 * q < HD) {
-            float v[2 * N];
+            float v[2 * N];  // weights' part, then their rests'
             tmem_ld_cols(oc, v);
             tmem_wait_ld();
 #pragma unroll
@@ -462,6 +481,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
     const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
     const int j = threadIdx.x;  // the key of a tile (n <= 32) or the query row (n > 32) of this thread
     float* mx_s = reinterpret_cast<float*>(smem + S::OFF_MX);
+    float *m_s = mx_s + 128, *a_s = m_s + 32;
     int i = 0, seg = 0;
     // Rows past the request's last: P is zero there, but what the cache holds may be NaN (past a prefix's end
     // the copy has already put zeros).
@@ -475,56 +495,66 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
           if (SK_INB(nk * 8 + u < 1024, p.err))
             *reinterpret_cast<uint4*>(Vt + ch * 16384 + nk * 128 + u * 16) = make_uint4(0, 0, 0, 0);
     };
-    // n <= 32 query rows, N of them in registers
-    auto by_keys = [&](auto half, int n) {
-      constexpr int N = decltype(half)::value;
-      float m[N], l[N];
-#pragma unroll
-      for (int h = 0; h < N; ++h) m[h] = -INFINITY, l[h] = 0.f;
+    // n <= 32 query rows: N the half width of the columns, H >= n rows computed
+    auto by_keys = [&](auto half, auto rows, int n) {
+      constexpr int N = decltype(half)::value, H = decltype(rows)::value;
+      float l[H] = {};
       const uint32_t o_at = tO + (seg & 1) * 128 + lane_off;
       float* sc = !sg.prefix && p.mass ? p.sc + ((long long)sg.r * p.nq + sg.kvh * p.g) * p.sc_stride + j : nullptr;
       for (int t = sg.t0; t < sg.t1; ++t, ++i) {
         const int w = i & 1, nk = min(CutTc::KT, sg.n_keys - t * CutTc::KT);
         wait(&s_full[w], i >> 1);
         tc_fence_after();
-        float x[2 * N];
-        tmem_ld_cols(tS + w * 128 + lane_off, x);
-        tmem_wait_ld();
-        bool over = false;
+        float x[H];
+        {
+          float raw[2 * N];
+          tmem_ld_cols(tS + w * 128 + lane_off, raw);
+          tmem_wait_ld();
 #pragma unroll
-        for (int h = 0; h < N; ++h) {
-          x[h] = j < nk && h < n ? x[h] + x[N + h] : -INFINITY;
-          over |= x[h] > m[h] + kRescale;
+          for (int h = 0; h < H; ++h) x[h] = j < nk && h < n ? raw[h] + raw[N + h] : -INFINITY;
+        }
+        bool over = t == sg.t0;
+        if (t > sg.t0) {
+#pragma unroll
+          for (int h = 0; h < H; ++h) over |= x[h] > m_s[h] + kRescale;
         }
         if (sc) {
 #pragma unroll
-          for (int h = 0; h < (N < kMaxGroup ? N : kMaxGroup); ++h)
+          for (int h = 0; h < (H < kMaxGroup ? H : kMaxGroup); ++h)
             if (h < n) sc[h * p.sc_stride + (long long)t * CutTc::KT] = x[h];
         }
         if (any_of_128(over)) {
+          float y[H];
 #pragma unroll
-          for (int h = 0; h < N; ++h) {
-            const float y = warp_max_f32(x[h]);
-            if (lane == 0) mx_s[warp * 32 + h] = y;
+          for (int h = 0; h < H; ++h) y[h] = x[h];
+          const float top = warp_reduce<H>(y, [](float a, float b) { return fmaxf(a, b); });
+          if (lane % (32 / H) == 0) mx_s[warp * 32 + lane / (32 / H)] = top;
+          named_bar_sync(2, 128);
+          if (j < H) {
+            const float old = t > sg.t0 ? m_s[j] : -INFINITY;
+            const float to = fmaxf(fmaxf(fmaxf(mx_s[j], mx_s[32 + j]), fmaxf(mx_s[64 + j], mx_s[96 + j])), old);
+            a_s[j] = to == -INFINITY ? 1.f : ex2_approx(old - to);
+            m_s[j] = to;
           }
           named_bar_sync(2, 128);
-          float a[N];
-#pragma unroll
-          for (int h = 0; h < N; ++h) {
-            const float y = fmaxf(fmaxf(fmaxf(mx_s[h], mx_s[32 + h]), fmaxf(mx_s[64 + h], mx_s[96 + h])), m[h]);
-            a[h] = y == -INFINITY ? 1.f : ex2_approx(m[h] - y);
-            l[h] *= a[h];
-            m[h] = y;
-          }
           if (t > sg.t0) {
+#pragma unroll
+            for (int h = 0; h < H; ++h) l[h] *= a_s[h];
             wait(&o_done[(i - 1) & 1], (i - 1) >> 1);
             tc_fence_after();
-            float v[2 * N];
-            tmem_ld_cols(o_at, v);
-            tmem_wait_ld();
+#pragma unroll 1
+            for (int part = 0; part < 2; ++part) {  // the weights' columns and their rests'
+              float v[N < 16 ? 16 : N];
+              tmem_ld_cols(o_at + part * N, v);
+              tmem_wait_ld();
 #pragma unroll
-            for (int h = 0; h < N; ++h) v[h] *= a[h], v[N + h] *= a[h];
-            tmem_st_cols(o_at, v);
+              for (int h = 0; h < H; ++h) {
+                v[h] *= a_s[h];
+                if (N < 16) v[N + h] *= a_s[h];
+              }
+              tmem_st_cols(o_at + part * N, v);
+              if (N < 16) break;  // both at once
+            }
             tmem_wait_st();
             tc_fence_before();
           }
@@ -532,9 +562,8 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
         uint8_t* Pt = smem + S::OFF_PT + w * S::PT_BYTES + (j >> 6) * 8192 + (j & 7) * 2;
         const int unit = (j & 63) >> 3;
 #pragma unroll
-        for (int h = 0; h < N; ++h) {
-          if (h >= n) break;
-          const float y = ex2_approx(x[h] - (m[h] == -INFINITY ? 0.f : m[h]));
+        for (int h = 0; h < H; ++h) {
+          const float top = m_s[h], y = ex2_approx(x[h] - (top == -INFINITY ? 0.f : top));
           l[h] += y;
           const __nv_bfloat16 b = __float2bfloat16_rn(y);
           const int at = h * 128 + ((unit ^ (h & 7)) << 4);  // N rows on: the same low bits
@@ -548,15 +577,14 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
       }
       if (seg >= 2) wait(&o_free[seg & 1], (seg - 2) >> 1);
       float* st = reinterpret_cast<float*>(ml_s + (seg & 1) * 128);
-#pragma unroll
-      for (int h = 0; h < N; ++h) {
-        if (h >= n) break;
-        const float y = warp_sum_f32(l[h]);
-        if (lane == 0) st[warp * 32 + h] = y;
-        if (j == h) st[128 + h] = m[h];
-      }
+      if (j < H) st[128 + j] = m_s[j];
+      const float sum = warp_reduce<H>(l, [](float a, float b) { return a + b; });
+      if (lane % (32 / H) == 0) st[warp * 32 + lane / (32 / H)] = sum;
       mbar_arrive(&ml_full[seg & 1]);
     };
+    // n > 32 query rows, one per thread. A tile's scores are read twice, a quarter of the columns at a time,
+    // for the maximum and for the weights, which go back over the quarter they came from (16 columns of bf16
+    // pairs, 16 of their rests): in registers a row would take 128.
     auto by_rows = [&](int n) {
       const bool any = warp * 32 < n;
       const uint32_t o_at = tO + (seg & 1) * 128 + lane_off;
@@ -567,28 +595,30 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
         wait(&s_full[w], i >> 1);
         tc_fence_after();
         if (any) {
-          float x[128];
-          tmem_ld_cols(s_at, x);
-          tmem_wait_ld();
-          if (nk < CutTc::KT) {
+          float m_new = m_run;
+#pragma unroll 1
+          for (int u = 0; u < 4; u += 2) {
+            float x[64];
+            tmem_ld_cols(s_at + u * 32, x);
+            tmem_wait_ld();
+            if (nk < CutTc::KT) {
 #pragma unroll
-            for (int e = 0; e < 128; ++e) x[e] = e < nk ? x[e] : -INFINITY;
-          }
-          float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
+              for (int e = 0; e < 64; ++e) x[e] = u * 32 + e < nk ? x[e] : -INFINITY;
+            }
+            float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
-          for (int e = 0; e < 128; e += 8) {
-            m0 = max3(m0, x[e], x[e + 1]);
-            m1 = max3(m1, x[e + 2], x[e + 3]);
-            m2 = max3(m2, x[e + 4], x[e + 5]);
-            m3 = max3(m3, x[e + 6], x[e + 7]);
+            for (int e = 0; e < 64; e += 4) {
+              m0 = max3(m0, x[e], x[e + 1]);
+              m1 = max3(m1, x[e + 2], x[e + 3]);
+            }
+            m_new = max3(m_new, m0, m1);
           }
-          const float m_new = fmaxf(m_run, fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)));
           if (__any_sync(0xffffffffu, m_new > m_run + kRescale)) {  // O and the sum of this warp's rows
             const float alpha = m_new == -INFINITY ? 1.f : ex2_approx(m_run - m_new);
             if (t > sg.t0) {
               wait(&o_done[(i - 1) & 1], (i - 1) >> 1);
               tc_fence_after();
-#pragma unroll
+#pragma unroll 1
               for (int ch = 0; ch < HD / 32; ++ch) {
                 float v[32];
                 tmem_ld32(o_at + ch * 32, v);
@@ -604,19 +634,29 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
           }
           const float use = m_run == -INFINITY ? 0.f : m_run;
           float l0 = 0.f, l1 = 0.f;
+#pragma unroll 1
+          for (int u = 0; u < 4; u += 2) {
+            float x[64];
+            tmem_ld_cols(s_at + u * 32, x);
+            tmem_wait_ld();
+            if (nk < CutTc::KT) {
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            uint32_t hi[16], lo[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float a = ex2_approx(x[32 * u + 2 * e] - use), b = ex2_approx(x[32 * u + 2 * e + 1] - use);
-              l0 += a;
-              l1 += b;
-              hi[e] = pack_bf16(a, b);
-              if (P_SPLIT) lo[e] = pack_bf16(lo_part(a, hi[e], 0), lo_part(b, hi[e], 1));
+              for (int e = 0; e < 64; ++e) x[e] = u * 32 + e < nk ? x[e] : -INFINITY;
             }
-            tmem_st16(s_at + u * 16, hi);
-            if (P_SPLIT) tmem_st16(s_at + 64 + u * 16, lo);
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+              uint32_t hi[16], lo[16];
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const float a = ex2_approx(x[32 * v + 2 * e] - use), b = ex2_approx(x[32 * v + 2 * e + 1] - use);
+                l0 += a;
+                l1 += b;
+                hi[e] = pack_bf16(a, b);
+                if (P_SPLIT) lo[e] = pack_bf16(lo_part(a, hi[e], 0), lo_part(b, hi[e], 1));
+              }
+              tmem_st16(s_at + (u + v) * 32, hi);
+              if (P_SPLIT) tmem_st16(s_at + (u + v) * 32 + 16, lo);
+            }
           }
           l_run += l0 + l1;
           tmem_wait_st();
@@ -632,10 +672,12 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
       const int n = rows_of(p, sg), form = form_of(n);
       if (form == 0)
         by_rows(n);
+      else if (n <= 2)
+        by_keys(std::integral_constant<int, 8>(), std::integral_constant<int, 2>(), n);
       else if (form == 8)
-        by_keys(std::integral_constant<int, 8>(), n);
+        by_keys(std::integral_constant<int, 8>(), std::integral_constant<int, 8>(), n);
       else
-        by_keys(std::integral_constant<int, 32>(), n);
+        by_keys(std::integral_constant<int, 32>(), std::integral_constant<int, 32>(), n);
     }
   }
   tc_fence_before();
