@@ -100,14 +100,14 @@ __global__ void __launch_bounds__(kSimtThreads) tiles_simt_kernel(const Params p
 
     for (int i = w; i < n_rows; i += kSimtThreads / 32) {
       const int r = sg.prefix ? (row0 + i) / p.g : sg.r, h = sg.prefix ? (row0 + i) % p.g : i;
-      float x[E] = {};
-      if (ls.len[r] >= 0) {
-        load_row<HD>(p.qkv, r * p.qkv_stride + (long long)(sg.kvh * p.g + h) * HD, p.qkv_bf16, x);
-        norm_rotate<HD>(x, p.qn, p.rope, ls.pos[r], p.eps);
+      float x[1][E];
+      RawRow<HD> raw[1];
+      raw[0].load(p.qkv, r * p.qkv_stride + (long long)(sg.kvh * p.g + h) * HD, p.qkv_bf16);
+      const int pos[1] = {ls.pos[r]};
+      norm_rotate_rows<HD, 1>(x, raw, p.qkv_bf16, pos, p.qn, p.rope, p.eps);
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[e] *= p.q_scale;
-      }
-      store_vec<E>(Qs + i * HD + lane * E, x);
+      for (int e = 0; e < E; ++e) x[0][e] *= p.q_scale;
+      store_vec<E>(Qs + i * HD + lane * E, x[0]);
     }
     if (t < RT) {
       m_s[t] = -INFINITY;
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(kSimtThreads) tiles_simt_kernel(const Params p
 constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32, kMassChunk = 1024;
 
 template <class Cut, typename T, int HD>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
+__global__ void __launch_bounds__(kJoinThreads, 5) join_kernel(const Params p) {
   constexpr int E = HD / 32, RT = Cut::RT, KT = Cut::KT;
   __shared__ float snew_s[kMaxGroup], M_s[kMaxGroup], iL_s[kMaxGroup];
   __shared__ __align__(16) float red_s[kJoinWarps][HD];
@@ -248,13 +248,15 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
   float m_run = -INFINITY, l_run = 0.f;
   if (h < p.g) {
     const int pos = (int)p.pos[r];
-    float q[E], k[E], v[E];
     const long long base = r * p.qkv_stride;
-    load_row<HD>(p.qkv, base + (long long)(kvh * p.g + h) * HD, p.qkv_bf16, q);
-    load_row<HD>(p.qkv, base + (long long)(p.nq + kvh) * HD, p.qkv_bf16, k);
-    load_row<HD>(p.qkv, base + (long long)(p.nq + p.nkv + kvh) * HD, p.qkv_bf16, v);
-    norm_rotate<HD>(q, p.qn, p.rope, pos, p.eps);
-    norm_rotate<HD>(k, p.kn, p.rope, pos, p.eps);
+    RawRow<HD> raw[3];
+    raw[0].load(p.qkv, base + (long long)(kvh * p.g + h) * HD, p.qkv_bf16);
+    raw[1].load(p.qkv, base + (long long)(p.nq + kvh) * HD, p.qkv_bf16);
+    raw[2].load(p.qkv, base + (long long)(p.nq + p.nkv + kvh) * HD, p.qkv_bf16);
+    float qk[2][E], v[E];
+    norm_rotate_qk<HD>(qk, raw, p.qkv_bf16, pos, p.qn, p.kn, p.rope, p.eps);
+    raw[2].values(p.qkv_bf16, v);
+    float (&q)[E] = qk[0], (&k)[E] = qk[1];
     float dot = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) {

@@ -280,47 +280,64 @@ __device__ __forceinline__ void store_vec(float* p, const float (&x)[E]) {
 // ---- head rows ------------------------------------------------------------------------------------
 // One warp holds a head row of HD elements, HD / 32 consecutive ones per lane; an element's partner in the
 // rotate-half rotation (d and d + HD/2) is then in lane ^ 16 at the same place.
+// A row as it lies in memory, and its values: apart, so that a branch on the type between loads does not wait
+// for the data of each.
+template <int HD>
+struct RawRow {
+  static constexpr int E = HD / 32;
+  uint32_t w[E];
+  __device__ __forceinline__ void load(const void* base, long long at, int is_bf16) {
+    const int lane = threadIdx.x & 31;
+    if (is_bf16) {
+      const __nv_bfloat16* p = reinterpret_cast<const __nv_bfloat16*>(base) + at + lane * E;
+      if constexpr (E == 4) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        w[0] = v.x, w[1] = v.y;
+      } else {
+        w[0] = *reinterpret_cast<const uint32_t*>(p);
+      }
+    } else {
+      const float* p = reinterpret_cast<const float*>(base) + at + lane * E;
+      if constexpr (E == 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(p);
+        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+      } else {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        w[0] = v.x, w[1] = v.y;
+      }
+    }
+  }
+  __device__ __forceinline__ void values(int is_bf16, float (&x)[E]) const {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      x[e] = __uint_as_float(is_bf16 ? (e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16) : w[e]);
+  }
+};
 template <int HD>
 __device__ __forceinline__ void load_row(const void* base, long long at, int is_bf16, float (&x)[HD / 32]) {
-  constexpr int E = HD / 32;
-  const int lane = threadIdx.x & 31;
-  if (is_bf16) {
-    const __nv_bfloat16* p = reinterpret_cast<const __nv_bfloat16*>(base) + at + lane * E;
-    uint32_t w[E / 2];
-    if constexpr (E == 4) {
-      const uint2 v = *reinterpret_cast<const uint2*>(p);
-      w[0] = v.x;
-      w[1] = v.y;
-    } else {
-      w[0] = *reinterpret_cast<const uint32_t*>(p);
-    }
-#pragma unroll
-    for (int e = 0; e < E / 2; ++e) {
-      x[2 * e] = __uint_as_float(w[e] << 16);
-      x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-    }
-  } else {
-    load_vec<E>(reinterpret_cast<const float*>(base) + at + lane * E, x);
-  }
+  RawRow<HD> r;
+  r.load(base, at, is_bf16);
+  r.values(is_bf16, x);
 }
 // RMS norm (x w) and rotation of B head rows in fp32, the reference's order of operations
-// (qwen3/kernels.py:354-380); row b turns by the table's row pos[r[b]]. Every load goes out before the first
+// (qwen3/kernels.py:354-380); row b turns by the table's row pos[b]. Every load goes out before the first
 // sum, and the rows' shuffles interleave.
 template <int HD, int B>
-__device__ __forceinline__ void norm_rotate_rows(float (&x)[B][HD / 32], const int (&r)[B], const int* pos,
-                                                 const float* w, const float* rope, float eps) {
+__device__ __forceinline__ void norm_rotate_rows(float (&x)[B][HD / 32], const RawRow<HD> (&raw)[B], int is_bf16,
+                                                 const int (&pos)[B], const float* w, const float* rope, float eps) {
   constexpr int E = HD / 32;
   const int lane = threadIdx.x & 31;
   float wv[E], c[B][E], s[B][E], ss[B];
   load_vec<E>(w + lane * E, wv);
 #pragma unroll
   for (int b = 0; b < B; ++b) {
-    const float* turn = rope + (long long)pos[r[b]] * HD + (lane & 15) * E;
+    const float* turn = rope + (long long)pos[b] * HD + (lane & 15) * E;
     load_vec<E>(turn, c[b]);
     load_vec<E>(turn + HD / 2, s[b]);
   }
 #pragma unroll
   for (int b = 0; b < B; ++b) {
+    raw[b].values(is_bf16, x[b]);
     ss[b] = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) ss[b] += x[b][e] * x[b][e];
@@ -340,10 +357,38 @@ __device__ __forceinline__ void norm_rotate_rows(float (&x)[B][HD / 32], const i
     }
   }
 }
+// The q row raw[0] (x qn) and the k row raw[1] (x kn) of one token.
 template <int HD>
-__device__ __forceinline__ void norm_rotate(float (&x)[HD / 32], const float* w, const float* rope, int pos, float eps) {
-  const int zero[1] = {0};
-  norm_rotate_rows<HD, 1>(reinterpret_cast<float (&)[1][HD / 32]>(x), zero, &pos, w, rope, eps);
+__device__ __forceinline__ void norm_rotate_qk(float (&x)[2][HD / 32], const RawRow<HD> (&raw)[3], int is_bf16, int pos,
+                                               const float* qn, const float* kn, const float* rope, float eps) {
+  constexpr int E = HD / 32;
+  const int lane = threadIdx.x & 31;
+  float wv[2][E], c[E], s[E], ss[2];
+  load_vec<E>(qn + lane * E, wv[0]);
+  load_vec<E>(kn + lane * E, wv[1]);
+  load_vec<E>(rope + (long long)pos * HD + (lane & 15) * E, c);
+  load_vec<E>(rope + (long long)pos * HD + HD / 2 + (lane & 15) * E, s);
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    raw[b].values(is_bf16, x[b]);
+    ss[b] = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) ss[b] += x[b][e] * x[b][e];
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int b = 0; b < 2; ++b) ss[b] += __shfl_xor_sync(0xffffffffu, ss[b], o);
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    const float inv = rsqrtf(ss[b] / HD + eps);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float y = x[b][e] * inv * wv[b][e];
+      const float other = __shfl_xor_sync(0xffffffffu, y, 16);
+      x[b][e] = y * c[e] + (lane < 16 ? -other : other) * s[e];
+    }
+  }
 }
 
 // shared_decode_tc.cu: the key tiles on the tensor cores (bf16 caches); p_split: the weights in two bf16 terms.
