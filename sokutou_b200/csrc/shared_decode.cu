@@ -77,19 +77,19 @@ __global__ void __launch_bounds__(kSimtThreads) tiles_simt_kernel(const Params p
   float* l_s = m_s + RT;
   float* a_s = l_s + RT;
   const Lens ls(smem + S::OFF_CUM, p.R);
-  __shared__ int any_s;
+  __shared__ Tiles tiles_s;
   const int t = threadIdx.x, lane = t & 31, w = t >> 5, c = blockIdx.x;
 
   griddep_wait();
   griddep_launch_dependents();
   if (w == 0) {
-    const bool any = scan_tiles<KT>(p, ls, c == 0);
-    if (lane == 0) any_s = any;
+    const Tiles t = scan_tiles<CutSimt>(p, ls, c == 0);
+    if (lane == 0) tiles_s = t;
   }
   __syncthreads();
-  const Tiles tl = tiles_of<CutSimt>(p, ls.cum[p.R], any_s);
+  const Tiles tl = tiles_s;
   Segments sg;
-  for (bool more = sg.first(p, tl, ls, c); more; more = sg.next(p, tl, ls)) {
+  for (bool more = sg.first<KT>(p, tl, ls, c); more; more = sg.next<KT>(p, tl, ls)) {
     const int row0 = sg.prefix ? sg.r * RT : 0;
     const int n_rows = sg.prefix ? min(RT, p.R * p.g - row0) : p.g;
     const T* Kb = sg.prefix ? reinterpret_cast<const T*>(p.Kp) + sg.kvh * p.prefix_head_stride
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(kJoinThreads, 5) join_kernel(const Params p) {
   __shared__ float snew_s[kMaxGroup], M_s[kMaxGroup], iL_s[kMaxGroup];
   __shared__ __align__(16) float red_s[kJoinWarps][HD];
   __shared__ float2 ml_s[kJoinWarps];
-  __shared__ int before_s[kJoinWarps], all_s[kJoinWarps];
+  __shared__ int4 sums_s[kJoinWarps];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int r = blockIdx.x / p.nkv, kvh = blockIdx.x % p.nkv;
   griddep_launch_dependents();
@@ -226,22 +226,25 @@ __global__ void __launch_bounds__(kJoinThreads, 5) join_kernel(const Params p) {
     griddep_wait();  // every thread, before any exit: the kernel after this one relies on it
     return;
   }
-  {  // own tiles of the requests before this one, and of all
-    int before = 0, all = 0;
+  {  // own tiles and items of the requests before this one, and of all
+    int4 v = make_int4(0, 0, 0, 0);
     for (int x = threadIdx.x; x < p.R; x += kJoinThreads) {
       const int k = own_rows(p, x, &bad), tiles = k > 0 ? (k + KT - 1) / KT : 0;
-      all += tiles;
-      if (x < r) before += tiles;
+      v.z += tiles;
+      v.w += k > 0;
+      if (x < r) {
+        v.x += tiles;
+        v.y += k > 0;
+      }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-      before += __shfl_xor_sync(0xffffffffu, before, o);
-      all += __shfl_xor_sync(0xffffffffu, all, o);
+      v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+      v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+      v.z += __shfl_xor_sync(0xffffffffu, v.z, o);
+      v.w += __shfl_xor_sync(0xffffffffu, v.w, o);
     }
-    if (lane == 0) {
-      before_s[w] = before;
-      all_s[w] = all;
-    }
+    if (lane == 0) sums_s[w] = v;
   }
   const int per = max(1, kJoinWarps / p.g), h = w / per, sub = w % per;  // warps per head
   float acc[E] = {};
@@ -282,24 +285,26 @@ __global__ void __launch_bounds__(kJoinThreads, 5) join_kernel(const Params p) {
     }
   }
   __syncthreads();
-  int before = 0, all = 0;
+  int4 sum = make_int4(0, 0, 0, 0);
 #pragma unroll
   for (int x = 0; x < kJoinWarps; ++x) {
-    before += before_s[x];
-    all += all_s[x];
+    const int4 v = sums_s[x];
+    sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
   }
-  const Tiles tl = tiles_of<Cut>(p, all, true);
+  const Tiles tl = tiles_of<Cut>(p, sum.z, sum.w, true);
   const int i = r * p.g + h, rt = i / RT, il = i - rt * RT;
   const int ip = kvh * tl.nrt + rt, io = r * p.nkv + kvh, tr = (n + KT - 1) / KT;
   int pc = 0, np = 0, oc = 0, no = 0;
   if (tl.tp > 0) {
-    pc = share_of(tl, ip * tl.tp);
-    np = share_of(tl, (ip + 1) * tl.tp - 1) - pc + 1;
+    const int at = ip * tl.cost_p();
+    pc = share_of(tl, at);
+    np = share_of(tl, at + start_of(tl.tp - 1, tl.first_p, tl.shift_p)) - pc + 1;
   }
   if (tr > 0) {
-    const int first = tl.n_prefix + before * p.nkv + kvh * tr;
-    oc = share_of(tl, first);
-    no = share_of(tl, first + tr - 1) - oc + 1;
+    const int at = tl.prefix + p.nkv * (sum.y * tl.first_o + (sum.x << tl.shift_o)) +
+                   kvh * (tl.first_o + (tr << tl.shift_o));
+    oc = share_of(tl, at);
+    no = share_of(tl, at + start_of(tr - 1, tl.first_o, tl.shift_o)) - oc + 1;
   }
   griddep_wait();
   if (h < p.g) {

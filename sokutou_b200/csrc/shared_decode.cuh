@@ -3,13 +3,14 @@
 //
 // Work. The keys of a step are cut into tiles of KT rows: first the prefix, per (key/value head, tile of RT
 // query rows) an item of ceil(P / KT) tiles — query row i = r*g + h of a head, all requests together —, then
-// the own rows, per (request, key/value head) an item of ceil(n / KT) tiles. All tiles in one row, item
-// after item, are split evenly over the CTAs, one more for the first N mod G: every CTA
-// moves the same number of bytes whatever the lengths are, and an item is cut only where a CTA's share
-// ends. The part of an item that one CTA does is a segment; it leaves one partial (running max, sum,
-// unnormalised output) per query row. Along the row of tiles the pair (CTA, item) never steps back in
-// either and moves in one at least, so CTA + item numbers a segment's place in the workspace uniquely.
-// The lengths are read on the device, so one captured graph serves every step.
+// the own rows, per (request, key/value head) an item of ceil(n / KT) tiles. All tiles lie in one row, item
+// after item, each at its cost from the start (see Tiles), and the row is cut into equal shares for the CTAs
+// of the grid, a tile falling to the share that its start lies in: every CTA has the same to do whatever
+// the lengths are, and an item is cut only where a share ends. The part of an item that one CTA does is a
+// segment; it leaves one partial (running max, sum, unnormalised output) per query row. Along the row the
+// pair (CTA, item) never steps back in either and moves in one at least, so CTA + item numbers a segment's
+// place in the workspace uniquely. The lengths are read on the device, so one captured graph serves every
+// step.
 #pragma once
 
 #include "sk_common.cuh"
@@ -56,17 +57,18 @@ struct Params {
 };
 
 // How one of the two main kernels cuts the work: key rows per tile, query rows per prefix item, CTAs.
-template <int KT_, int RT_, int G_>
+template <int KT_, int RT_, int G_, bool kWeighted_>
 struct CutOf {
   static constexpr int KT = KT_, RT = RT_, G = G_;
+  static constexpr bool kWeighted = kWeighted_;
 };
-using CutSimt = CutOf<64, 16, 296>;   // CUDA cores: two CTAs on each of 148 SMs
-using CutTc = CutOf<128, 128, 148>;   // tensor cores: one CTA on each
-// All tiles of a step at the most (2^31 and above are refused).
+using CutSimt = CutOf<64, 16, 296, false>;   // CUDA cores: two CTAs on each of 148 SMs
+using CutTc = CutOf<128, 128, 148, true>;    // tensor cores: one CTA on each
+// All tiles of a step at the most, at the highest cost (2^31 and above are refused).
 template <class Cut>
 __host__ inline bool too_many_tiles(long long R, long long g, long long nkv, long long P, long long max_len) {
   const long long tp = (P + Cut::KT - 1) / Cut::KT, to = (max_len + Cut::KT - 1) / Cut::KT;
-  return nkv * (tp * ((R * g + Cut::RT - 1) / Cut::RT) + R * to) > 0x7fffffffLL;
+  return nkv * (tp * ((R * g + Cut::RT - 1) / Cut::RT) + R * to) > 0x7fffffffLL / 8;
 }
 
 __host__ __device__ inline long long align_up(long long x, long long a) { return (x + a - 1) / a * a; }
@@ -107,113 +109,160 @@ __device__ __forceinline__ int own_rows(const Params& p, int r, bool* bad) {
   return (int)n;
 }
 
-// One warp: for every request its own tiles per head before it (cum[R]: of all), its own rows (-1: idle) and
-// its position; whether any is live; records positions out of range.
-struct Lens {  // shared memory, kMaxRequests-bounded
-  int* cum;    // [R + 1]
+// The row of tiles of one step (the host refuses sizes whose costs could pass 2^31). With many tiles a CTA
+// each tile costs 2^shift and the first of an item `first` more: a segment's query rows have to be read,
+// normalised and written as an operand, and its partials drained. On the tensor cores: own tiles 2, 2 more for
+// the first; prefix tiles of more than kFewRows query rows 4, 4 more for the first (they take the tensor cores
+// and the exponentials for about twice as long, and their rows are many; with every tile at 1 the prefix's
+// CTAs took 133 thousand cycles when the others took 75, at 64 requests behind 8192 rows). With fewer tiles
+// each costs 1 and is a CTA's own.
+constexpr int kFewRows = 8;
+
+struct Tiles {
+  int tp, nrt;         // tiles of a prefix item; prefix items per head
+  int items_p;         // prefix items
+  int shift_p, first_p, shift_o, first_o;
+  int prefix;          // cost of all prefix items
+  int each, more;      // a share costs `each`, one more for the first `more` CTAs
+  __device__ __forceinline__ int cost_p() const { return first_p + (tp << shift_p); }
+};
+// own_tiles, own_items: of all requests, per head.
+template <class Cut>
+__device__ __forceinline__ Tiles tiles_of(const Params& p, int own_tiles, int own_items, bool any) {
+  Tiles t;
+  const int rows = p.R * p.g;
+  t.tp = any ? (int)((uint32_t)(p.P + Cut::KT - 1) / Cut::KT) : 0;
+  t.nrt = (int)((uint32_t)(rows + Cut::RT - 1) / Cut::RT);
+  t.items_p = t.tp > 0 ? t.nrt * p.nkv : 0;
+  const bool many = rows > kFewRows;
+  t.shift_o = 1, t.first_o = 2;
+  t.shift_p = many ? 2 : 1, t.first_p = many ? 4 : 2;
+  int total = t.items_p * t.cost_p() + p.nkv * (own_items * t.first_o + (own_tiles << t.shift_o));
+  // no share may be without a tile's start: a share costs at least what lies between two starts
+  if (!Cut::kWeighted || total < Cut::G * (t.items_p && many ? 8 : 4)) {
+    t.shift_o = t.first_o = t.shift_p = t.first_p = 0;
+    total = t.items_p * t.tp + p.nkv * own_tiles;
+  }
+  t.prefix = t.items_p * t.cost_p();
+  t.each = (int)((uint32_t)total / Cut::G);
+  t.more = total - t.each * Cut::G;
+  return t;
+}
+__device__ __forceinline__ int share_begin(const Tiles& t, int c) { return c * t.each + min(c, t.more); }
+__device__ __forceinline__ int share_of(const Tiles& t, int at) {  // the CTA whose share holds cost position `at`
+  const uint32_t cut = (uint32_t)t.more * (t.each + 1);
+  return (int)((uint32_t)at < cut ? (uint32_t)at / (t.each + 1) : t.more + ((uint32_t)at - cut) / t.each);
+}
+// Where tile x of an item starts, from the item's start.
+__device__ __forceinline__ int start_of(int x, int first, int shift) { return x > 0 ? first + (x << shift) : 0; }
+
+// Own rows (-1: idle), position and cost of the requests before, per request.
+struct Lens {  // in shared memory
+  int* cum;    // [R + 1] cost per head of the own rows of the requests before r
   int* len;    // [R]
   int* pos;    // [R]
   static __host__ __device__ int bytes(int R) { return (3 * R + 1) * 4; }
   __device__ __forceinline__ Lens(void* at, int R) : cum((int*)at), len(cum + R + 1), pos(len + R) {}
 };
-template <int KT>
-__device__ __forceinline__ bool scan_tiles(const Params& p, const Lens& s, bool report) {
+// One warp: fills `s` and returns the row of tiles; records positions out of range.
+template <class Cut>
+__device__ __forceinline__ Tiles scan_tiles(const Params& p, const Lens& s, bool report) {
+  constexpr int KT = Cut::KT;
   const int lane = threadIdx.x & 31;
+  bool bad = false;
+  int tiles = 0, items = 0, live = 0;
+#pragma unroll 4
+  for (int r = lane; r < p.R; r += 32) {  // no iteration waits for another's loads
+    const int n = own_rows(p, r, &bad);
+    s.len[r] = n;
+    s.pos[r] = n >= 0 ? (int)p.pos[r] : 0;
+    tiles += n > 0 ? (n + KT - 1) / KT : 0;
+    items += n > 0;
+    live += n >= 0;
+  }
+  if (report && bad) set_dev_error(p.err, SK_DEVERR_POS_RANGE);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+    items += __shfl_xor_sync(0xffffffffu, items, o);
+  }
+  const Tiles t = tiles_of<Cut>(p, tiles, items, __any_sync(0xffffffffu, live > 0));
   int base = 0;
-  bool any = false, bad = false;
+  __syncwarp();
+#pragma unroll 1
   for (int r0 = 0; r0 < p.R; r0 += 32) {
-    const int r = r0 + lane;
-    const int n = r < p.R ? own_rows(p, r, &bad) : -1;
-    any |= n >= 0;
-    int x = n > 0 ? (n + KT - 1) / KT : 0;
-    const int own = x;
+    const int r = r0 + lane, n = r < p.R ? s.len[r] : 0;
+    const int own = n > 0 ? t.first_o + (((n + KT - 1) / KT) << t.shift_o) : 0;
+    int x = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, x, o);
       if (lane >= o) x += y;
     }
-    if (r < p.R) {
-      s.cum[r] = base + x - own;
-      s.len[r] = n;
-      s.pos[r] = n >= 0 ? (int)p.pos[r] : 0;
-    }
+    if (r < p.R) s.cum[r] = base + x - own;
     base += __shfl_sync(0xffffffffu, x, 31);
   }
   if (lane == 0) s.cum[p.R] = base;
-  if (report && bad) set_dev_error(p.err, SK_DEVERR_POS_RANGE);
-  return __any_sync(0xffffffffu, any);
-}
-
-// The row of tiles of one step (the host refuses sizes with 2^31 tiles).
-struct Tiles {
-  int tp;          // tiles of a prefix item
-  int nrt;         // prefix items per head
-  int n_prefix;    // tiles of all prefix items
-  int n;           // all tiles
-  int each, more;  // a share is `each` tiles, one more for the first `more` CTAs
-};
-template <class Cut>
-__device__ __forceinline__ Tiles tiles_of(const Params& p, int own_tiles, bool any) {
-  Tiles t;
-  t.tp = any ? (int)((uint32_t)(p.P + Cut::KT - 1) / Cut::KT) : 0;
-  t.nrt = (int)((uint32_t)(p.R * p.g + Cut::RT - 1) / Cut::RT);
-  t.n_prefix = t.tp * t.nrt * p.nkv;
-  t.n = t.n_prefix + own_tiles * p.nkv;
-  t.each = (int)((uint32_t)t.n / Cut::G);
-  t.more = t.n - t.each * Cut::G;
+  __syncwarp();
   return t;
-}
-__device__ __forceinline__ int share_begin(const Tiles& t, int c) { return c * t.each + min(c, t.more); }
-__device__ __forceinline__ int share_of(const Tiles& t, int tile) {  // the CTA whose share holds `tile`
-  const uint32_t cut = (uint32_t)t.more * (t.each + 1);
-  return (int)((uint32_t)tile < cut ? (uint32_t)tile / (t.each + 1) : t.more + ((uint32_t)tile - cut) / t.each);
 }
 
 // The segments of a CTA's share, one after another.
 struct Segments {
   bool prefix;
-  int item;        // prefix: kvh * nrt + rt; own: r * nkv + kvh
-  int kvh, r;      // r: request (own), or the tile of query rows (prefix)
-  int t0, t1;      // tiles of the item
-  int n_keys;      // rows of the item (prefix: P; own: n)
-  int left;        // tiles of the share after this segment
+  int item;     // prefix: kvh * nrt + rt; own: r * nkv + kvh
+  int kvh, r;   // r: request (own), or the tile of query rows (prefix)
+  int t0, t1;   // tiles of the item
+  int n_keys;   // rows of the item (prefix: P; own: n)
+  int at, end;  // cost positions of the item's start and of the share's end
 
   // The first segment of CTA c's share; false: the share is empty.
+  template <int KT>
   __device__ __forceinline__ bool first(const Params& p, const Tiles& t, const Lens& s, int c) {
-    const int tile = share_begin(t, c);
-    left = share_begin(t, c + 1) - tile;
-    if (left <= 0) return false;
-    if (tile < t.n_prefix) {
+    const int from = share_begin(t, c);
+    end = share_begin(t, c + 1);
+    if (from >= end) return false;
+    int off, tiles, shift, extra;
+    if (from < t.prefix) {
+      const int cost = t.cost_p();
       prefix = true;
-      item = (int)((uint32_t)tile / t.tp);
+      item = (int)((uint32_t)from / cost);
       kvh = (int)((uint32_t)item / t.nrt);
       r = item - kvh * t.nrt;
-      t0 = tile - item * t.tp;
-      take(t.tp, p.P);
-      return true;
+      at = item * cost;
+      n_keys = p.P;
+      tiles = t.tp, shift = t.shift_p, extra = t.first_p;
+    } else {
+      const int o = from - t.prefix;
+      int lo = 0, hi = p.R;  // the last r with cum[r] * nkv <= o: it has tiles
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s.cum[mid] * p.nkv <= o)
+          lo = mid;
+        else
+          hi = mid;
+      }
+      const int cost = s.cum[lo + 1] - s.cum[lo], in_r = o - s.cum[lo] * p.nkv;
+      prefix = false;
+      r = lo;
+      kvh = (int)((uint32_t)in_r / cost);
+      item = lo * p.nkv + kvh;
+      at = from - (in_r - kvh * cost);
+      n_keys = s.len[lo];
+      tiles = (n_keys + KT - 1) / KT, shift = t.shift_o, extra = t.first_o;
     }
-    const int o = tile - t.n_prefix;
-    int lo = 0, hi = p.R;  // the last r with cum[r] * nkv <= o: it has tiles
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (s.cum[mid] * p.nkv <= o)
-        lo = mid;
-      else
-        hi = mid;
-    }
-    const int tr = s.cum[lo + 1] - s.cum[lo];
-    const int in_r = o - s.cum[lo] * p.nkv;
-    prefix = false;
-    r = lo;
-    kvh = (int)((uint32_t)in_r / tr);
-    item = lo * p.nkv + kvh;
-    t0 = in_r - kvh * tr;
-    take(tr, s.len[lo]);
+    off = from - at;
+    // the first tile that starts at `off` or later; past the item's last: the next item's first
+    t0 = off == 0 ? 0 : max(1, (off - extra + (1 << shift) - 1) >> shift);
+    if (t0 >= tiles) return next<KT>(p, t, s);
+    take(tiles, extra, shift);
     return true;
   }
   // Steps on; false after the last. Items follow one another without gaps, so no division is needed.
+  template <int KT>
   __device__ __forceinline__ bool next(const Params& p, const Tiles& t, const Lens& s) {
-    if (left <= 0) return false;
+    at += prefix ? t.cost_p() : s.cum[r + 1] - s.cum[r];
+    if (at >= end) return false;
     t0 = 0;
     if (prefix) {
       if (++r == t.nrt) {
@@ -222,7 +271,7 @@ struct Segments {
       }
       ++item;
       if (kvh < p.nkv) {
-        take(t.tp, p.P);
+        take(t.tp, t.first_p, t.shift_p);
         return true;
       }
       prefix = false;
@@ -235,15 +284,14 @@ struct Segments {
       while (s.len[r] <= 0);  // a request with tiles follows, as the share goes on
     }
     item = r * p.nkv + kvh;
-    take(s.cum[r + 1] - s.cum[r], s.len[r]);
+    n_keys = s.len[r];
+    take((n_keys + KT - 1) / KT, t.first_o, t.shift_o);
     return true;
   }
 
  private:
-  __device__ __forceinline__ void take(int tiles, int keys) {
-    n_keys = keys;
-    t1 = min(tiles, t0 + left);
-    left -= t1 - t0;
+  __device__ __forceinline__ void take(int tiles, int extra, int shift) {  // those that start before the end
+    t1 = min(tiles, max(1, (end - at - extra + (1 << shift) - 1) >> shift));
   }
 };
 

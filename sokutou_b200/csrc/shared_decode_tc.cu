@@ -38,7 +38,7 @@ constexpr int kWarpB = 4, kWarpQo = 8, kWarpProducer = 12, kWarpS = 13, kWarpPv 
 constexpr int kLaunchRegs = 104, kSoftmaxRegs = 128, kQoRegs = 104, kControlRegs = 56;
 static_assert(128 * (2 * kSoftmaxRegs + kQoRegs + kControlRegs) <= kThreadsTc * kLaunchRegs, "register split over budget");
 constexpr float kRescale = 8.0f;  // O is rescaled when the running max grows by more than 2^8; exact either way
-constexpr int kFew = 8;           // query rows up to which the keys are the products' rows
+constexpr int kFew = kFewRows;    // query rows up to which the keys are the products' rows
 
 template <int N>
 __device__ __forceinline__ void setmaxnreg_inc() {
@@ -91,9 +91,9 @@ struct SmemTc {
   static constexpr int NBAR = 2 * NSK + 2 * NSV + 16;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;    // tensor-memory base, whether there is a segment
   static constexpr int OFF_TILES = OFF_MISC + 16;
-  static constexpr int OFF_SEG = OFF_TILES + 32;
-  static constexpr int OFF_LENS = OFF_SEG + 32;
-  static_assert(sizeof(Tiles) <= 32 && sizeof(Segments) <= 32, "their places in shared memory");
+  static constexpr int OFF_SEG = OFF_TILES + 48;
+  static constexpr int OFF_LENS = OFF_SEG + 48;
+  static_assert(sizeof(Tiles) <= 48 && sizeof(Segments) <= 48, "their places in shared memory");
   static __host__ __device__ int bytes(int R) { return OFF_LENS + Lens::bytes(R); }
   static_assert(OFF_QT % 1024 == 0 && OFF_PT % 1024 == 0 && OFF_V % 1024 == 0, "swizzled tiles lie on 1024 bytes");
   static_assert(OFF_LENS + (3 * kMaxRequests + 1) * 4 <= 232448, "shared memory over the 227 KB per-CTA limit");
@@ -188,6 +188,10 @@ __device__ __forceinline__ int rows_of(const Params& p, const Segments& s) {
   return s.prefix ? min(CutTc::RT, p.R * p.g - s.r * CutTc::RT) : p.g;
 }
 
+// The operand's first row of a segment of n > 8 query rows: segments of up to 64 alternate between its halves,
+// so that one's rows can be written while the other's are read (the rest of a product is ignored).
+__device__ __forceinline__ int base_of(int n, int seg) { return n <= 64 ? 64 * (seg & 1) : 0; }
+
 template <int HD, bool P_SPLIT>
 __global__ void __maxnreg__(kLaunchRegs)
     tiles_tc_kernel(const __grid_constant__ CUtensorMap tmKp, const __grid_constant__ CUtensorMap tmVp,
@@ -242,12 +246,10 @@ __global__ void __maxnreg__(kLaunchRegs)
   griddep_wait();
   griddep_launch_dependents();
   if (warp == kWarpScan) {
-    const bool any = scan_tiles<CutTc::KT>(p, ls, c == 0);
-    __syncwarp();
+    const Tiles tl = scan_tiles<CutTc>(p, ls, c == 0);
     if (lane == 0) {
-      const Tiles tl = tiles_of<CutTc>(p, ls.cum[p.R], any);
       Segments sg;
-      misc[1] = sg.first(p, tl, ls, c);
+      misc[1] = sg.first<CutTc::KT>(p, tl, ls, c);
       *reinterpret_cast<Tiles*>(smem + S::OFF_TILES) = tl;
       *reinterpret_cast<Segments*>(smem + S::OFF_SEG) = sg;
     }
@@ -273,6 +275,7 @@ __global__ void __maxnreg__(kLaunchRegs)
     const int n = rows_of(p, s);
     const bool few = n <= kFew;
     constexpr int kRowsAhead = 4;
+    const int base = few ? 0 : base_of(n, seg);
 #pragma unroll 1
     for (int i0 = first; i0 < n; i0 += step * kRowsAhead) {
       RawRow<HD> raw[kRowsAhead];
@@ -299,7 +302,7 @@ __global__ void __maxnreg__(kLaunchRegs)
         }
         // element d: 64-element chunk d / 64, 16-byte unit (d % 64) / 8 exclusive-or the row's low bits
         const int d = lane * E, unit = (d & 63) >> 3, chunk = d >> 6;
-        const int in_row = i * 128 + ((unit ^ (i & 7)) << 4) + (d & 7) * 2;
+        const int in_row = (base + i) * 128 + ((unit ^ (i & 7)) << 4) + (d & 7) * 2;
         const int at_hi = few ? S::OFF_QT + (seg & 1) * S::QT_BYTES + chunk * 2048 + in_row : S::OFF_Q + chunk * 16384 + in_row;
         const int at_lo = at_hi + (few ? kFew * 128 : S::Q_BYTES);
         if (SK_INB(at_lo + 2 * E <= S::OFF_PT, p.err)) {
@@ -322,7 +325,7 @@ __global__ void __maxnreg__(kLaunchRegs)
       // ---------------------------------------------------------------- TMA producer
       int i = 0;
       bool ok = true;
-      for (; more && ok; more = sg.next(p, tl, ls)) {
+      for (; more && ok; more = sg.next<CutTc::KT>(p, tl, ls)) {
         const MapOrder& o = args.order;
         for (int t = sg.t0; t < sg.t1 && ok; ++t, ++i) {
           // K, then V of the tile (one copy of the code: what(0), what(1))
@@ -360,7 +363,7 @@ __global__ void __maxnreg__(kLaunchRegs)
       const uint64_t k0 = smem_desc_sw128(sbase + S::OFF_K, 16, 1024);
       int i = 0, seg = 0;
       bool ok = true;
-      for (; more && ok; more = sg.next(p, tl, ls), ++seg) {
+      for (; more && ok; more = sg.next<CutTc::KT>(p, tl, ls), ++seg) {
         const bool few = rows_of(p, sg) <= kFew;
         if (!(ok = wait_on(&q_full[seg & 1], seg >> 1, p.err))) break;
         for (int t = sg.t0; t < sg.t1; ++t, ++i) {
@@ -396,7 +399,7 @@ __global__ void __maxnreg__(kLaunchRegs)
       const uint64_t v0 = smem_desc_sw128(sbase + S::OFF_V, 16384, 1024), p0 = smem_desc_sw128(sbase + S::OFF_PT, 16, 1024);
       int i = 0, seg = 0;
       bool ok = true;
-      for (; more && ok; more = sg.next(p, tl, ls), ++seg) {
+      for (; more && ok; more = sg.next<CutTc::KT>(p, tl, ls), ++seg) {
         const bool few = rows_of(p, sg) <= kFew;
         const uint32_t oc = tO + (seg & 1) * 128;
         if (seg >= 2 && !(ok = wait_on(&o_free[seg & 1], (seg - 2) >> 1, p.err))) break;
@@ -435,8 +438,10 @@ __global__ void __maxnreg__(kLaunchRegs)
     bool another = more;
     for (int s = 0; more; ++s) {
       if (another) {
-        // few rows alternate between two buffers; many have one, free once the scores before are done
-        if (s > 0 && rows_of(p, sg) > kFew && rows_of(p, nx) > kFew) wait(&sq_done[(s - 1) & 1], (s - 1) >> 1);
+        // up to 8 rows alternate between two buffers, up to 64 between two halves of one; where more are
+        // involved, the scores before have to be done
+        const int n0 = rows_of(p, sg), n1 = rows_of(p, nx);
+        if (s > 0 && min(n0, n1) > kFew && max(n0, n1) > 64) wait(&sq_done[(s - 1) & 1], (s - 1) >> 1);
         prepare(nx, s, s == 0 ? warp : q, s == 0 ? 12 : 4);
         if (s == 0) named_bar_sync(4, 384);
         if (warp < kWarpQo) break;
@@ -453,21 +458,24 @@ __global__ void __maxnreg__(kLaunchRegs)
         float2* ml = reinterpret_cast<float2*>(sg.prefix ? p.pml : p.oml) + row0;
         const float* st = reinterpret_cast<const float*>(smem + S::OFF_ML) + (seg & 1) * S::ML_FLOATS;
         const uint32_t oc = tO + (seg & 1) * 128 + ((uint32_t)(32 * q) << 16);
-        const int l = 32 * q + lane;
+        int l = 32 * q + lane;
         if (n > kFew) {
-          if (32 * q < n) {
+          const int base = base_of(n, seg);
+          l -= base;
+          if (32 * q < base + n && 32 * q + 32 > base) {
 #pragma unroll 1
             for (int ch = 0; ch < HD / 32; ++ch) {
               float v[32];
               tmem_ld32(oc + ch * 32, v);
               tmem_wait_ld();
-              if (l < n) {
+              if (l >= 0 && l < n) {
 #pragma unroll
                 for (int e = 0; e < 32; e += 4)
                   *reinterpret_cast<float4*>(o + l * HD + ch * 32 + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
               }
             }
-            if (l < n) ml[l] = make_float2(st[2 * l], st[2 * l + 1] + st[256 + l]);
+            if (l >= 0 && l < n)
+              ml[l] = make_float2(st[2 * (base + l)], st[2 * (base + l) + 1] + st[256 + base + l]);
           }
         } else {
           if (32 * q < HD) {  // lane l holds element l of every row
@@ -485,7 +493,7 @@ __global__ void __maxnreg__(kLaunchRegs)
         sg = nx;
         more = another;
       }
-      if (another) another = nx.next(p, tl, ls);
+      if (another) another = nx.next<CutTc::KT>(p, tl, ls);
     }
     if (warp < kWarpQo) {
       // ---------------------------------------------------------------- softmax
@@ -590,7 +598,8 @@ __global__ void __maxnreg__(kLaunchRegs)
       };
       // n > 8 query rows, row j; this thread's half of a tile's keys from column 64 * is_b
       auto by_rows = [&](int n) {
-        const bool any = (warp & 3) * 32 < n;
+        const int base = base_of(n, seg);
+        const bool any = (warp & 3) * 32 < base + n && (warp & 3) * 32 + 32 > base;
         const uint32_t o_at = tO + (seg & 1) * 128 + lane_off + is_b * (HD / 2);
         float m_run = -INFINITY, l_run = 0.f;
         for (int t = sg.t0; t < sg.t1; ++t, ++i) {
@@ -679,7 +688,7 @@ __global__ void __maxnreg__(kLaunchRegs)
         else
           *reinterpret_cast<float2*>(st + 2 * j) = make_float2(m_run, l_run);
       };
-      for (; more; more = sg.next(p, tl, ls), ++seg) {
+      for (; more; more = sg.next<CutTc::KT>(p, tl, ls), ++seg) {
         const int n = rows_of(p, sg);
         if (n > kFew) {
           by_rows(n);
