@@ -452,6 +452,11 @@ static int launch_tc(const Params& p, bool p_split, cudaStream_t st) {
   return rc != SK_OK ? rc : launch_join<CutTc, __nv_bfloat16, HD>(p, st);
 }
 
+// Whether every request reads the prefix for itself.
+static bool use_direct(const Params& p, int row_bytes) {
+  return (long long)p.R * p.nkv * p.P * 2 * row_bytes <= (p.f32 ? 64LL : 16LL) << 20;
+}
+
 static WsLayout layout_of(const SkSharedDecode* d) {
   return d->cache_dtype == SK_BF16
              ? ws_layout<CutTc>(d->R, d->nq, d->nkv, d->hd, d->prefix_len, d->max_len, d->mass != nullptr)
@@ -513,7 +518,7 @@ extern "C" int sk_decode_attention_shared(const SkSharedDecode* d, const void* q
   p.qkv_stride = d->qkv_stride, p.out_stride = d->out_stride;
   p.R = d->R, p.nq = d->nq, p.nkv = d->nkv, p.g = d->nq / d->nkv;
   p.P = d->prefix_len, p.max_len = d->max_len, p.rope_len = d->rope_len;
-  p.qkv_bf16 = q16, p.out_bf16 = o16;
+  p.f32 = d->cache_dtype == SK_F32, p.qkv_bf16 = q16, p.out_bf16 = o16;
   p.eps = d->eps;
   p.q_scale = (d->scale > 0.f ? d->scale : (hd == 128 ? 0.08838834764831845f : 0.125f)) * kLog2e;
   uint8_t* ws = reinterpret_cast<uint8_t*>(d->workspace);
@@ -523,6 +528,7 @@ extern "C" int sk_decode_attention_shared(const SkSharedDecode* d, const void* q
   p.err = sk_error_word_ptr();
   if (!p.err) return SK_ERR_CUDA;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (use_direct(p, hd * esz)) return launch_direct(p, hd, d->cache_dtype, st);
   if (d->cache_dtype == SK_BF16)
     return hd == 128 ? launch_tc<128>(p, !o16, st) : launch_tc<64>(p, !o16, st);
   return hd == 128 ? launch_simt<float, 128>(p, st) : launch_simt<float, 64>(p, st);

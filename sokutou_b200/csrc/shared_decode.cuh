@@ -45,7 +45,7 @@ struct Params {
   void* out;
   long long qkv_stride, out_stride;
   int R, nq, nkv, g, P, max_len, rope_len;
-  int qkv_bf16, out_bf16;
+  int f32, qkv_bf16, out_bf16;  // types of the caches, qkv and out
   float eps, q_scale;  // softmax scale * log2(e): scores come out in the log2 domain
   float* po;           // prefix partials [CTA + item][RT][hd]; ml [..][RT][2]
   float* pml;
@@ -441,6 +441,8 @@ __device__ __forceinline__ void norm_rotate_qk(float (&x)[2][HD / 32], const Raw
 
 // shared_decode_tc.cu: the key tiles on the tensor cores (bf16 caches); p_split: the weights in two bf16 terms.
 int launch_tiles_tc(const Params& p, int hd, bool p_split, cudaStream_t st);
+// shared_decode_direct.cu: every request for itself, in one launch.
+int launch_direct(const Params& p, int hd, int cache_dtype, cudaStream_t st);
 
 }  // namespace shared
 }  // namespace sk
