@@ -452,9 +452,16 @@ static int launch_tc(const Params& p, bool p_split, cudaStream_t st) {
   return rc != SK_OK ? rc : launch_join<CutTc, __nv_bfloat16, HD>(p, st);
 }
 
-// Whether every request reads the prefix for itself.
+// Whether every request reads the prefix for itself, in one launch. What that reads in all, against what the
+// two launches that share the prefix cost before their first byte and per request. Measured on both sides
+// (graph, 16 query over 8 key/value heads of 128, own rows 20 / 300 / 1000): at 16 requests it is 11.5 / 13.5 / 19.5 us
+// against 13.2 / 15.2 / 21.8 shared behind 512 rows (34 MB), 15.6 / 17.7 / 23.5 against 13.8 / 16.0 / 21.5
+// behind 1024 (67 MB); at one request 8.6 against 10.9 us behind 2048 rows and 18.4 against 13.6 behind 8192
+// (34 MB); at 64 requests 28 / 38 / 65 against 34 / 54 / 81 behind 512 (134 MB). fp32 caches have no tensor cores
+// to share rows on: 61 against 74 us for 16 requests behind 4096 rows (537 MB).
 static bool use_direct(const Params& p, int row_bytes) {
-  return (long long)p.R * p.nkv * p.P * 2 * row_bytes <= (p.f32 ? 64LL : 16LL) << 20;
+  const long long heads = (long long)p.R * p.nkv, mb = 1 << 20;
+  return heads * p.P * 2 * row_bytes <= (p.f32 ? 1024 * mb : 12 * mb + heads * mb / 3);
 }
 
 static WsLayout layout_of(const SkSharedDecode* d) {
@@ -528,7 +535,7 @@ extern "C" int sk_decode_attention_shared(const SkSharedDecode* d, const void* q
   p.err = sk_error_word_ptr();
   if (!p.err) return SK_ERR_CUDA;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (use_direct(p, hd * esz)) return launch_direct(p, hd, d->cache_dtype, st);
+  if (use_direct(p, hd * esz)) return launch_direct(p, hd, st);
   if (d->cache_dtype == SK_BF16)
     return hd == 128 ? launch_tc<128>(p, !o16, st) : launch_tc<64>(p, !o16, st);
   return hd == 128 ? launch_simt<float, 128>(p, st) : launch_simt<float, 64>(p, st);

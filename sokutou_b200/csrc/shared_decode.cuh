@@ -27,6 +27,22 @@ __device__ __forceinline__ void griddep_launch_dependents() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
+// mbar_wait in as few instructions as it takes: the kernel has some twenty waits, and its start is bound by
+// instruction fetches.
+__device__ __forceinline__ bool wait_on(uint64_t* bar, int phase, int* err) {
+  uint64_t t0 = 0;
+  for (uint32_t i = 1; !mbar_try_wait_sleep(bar, phase & 1); ++i) {
+    if (i & 15) continue;
+    const uint64_t now = globaltimer_ns();
+    if (t0 == 0) t0 = now;
+    if (now - t0 > kWaitLimitNs) {
+      set_dev_error(err, SK_DEVERR_TIMEOUT);
+      return false;
+    }
+  }
+  return true;
+}
+
 struct Params {
   const void* Kp;
   const void* Vp;
@@ -442,7 +458,7 @@ __device__ __forceinline__ void norm_rotate_qk(float (&x)[2][HD / 32], const Raw
 // shared_decode_tc.cu: the key tiles on the tensor cores (bf16 caches); p_split: the weights in two bf16 terms.
 int launch_tiles_tc(const Params& p, int hd, bool p_split, cudaStream_t st);
 // shared_decode_direct.cu: every request for itself, in one launch.
-int launch_direct(const Params& p, int hd, int cache_dtype, cudaStream_t st);
+int launch_direct(const Params& p, int hd, cudaStream_t st);
 
 }  // namespace shared
 }  // namespace sk

@@ -1,35 +1,31 @@
 // Shared-prefix decode attention in one launch, for steps where the prefix is short or the requests are few:
 // every (request, key/value head) reads prefix and own rows for itself (the prefix comes from L2 after the
-// first). A cluster of CTAs per (request, head), all rows dealt out to its warps in batches:
+// first). A cluster of CTAs per (request, head); the rows are dealt out to its warps in batches, straight from
+// global memory into registers. Warps are joined through shared memory, CTAs through the cluster's. The
+// running maximum is a warp's and moves only when a score exceeds it by 2^8.
 //
-//   A row is loaded as 16 bytes per lane, so a row takes W = 8, 16 or 32 lanes and one load of a warp covers
-//   32 / W rows; kLoads loads of K and of V make a batch, and the next batch is in flight while one is worked
-//   on. Scores: every lane multiplies its elements for all g heads, then one butterfly leaves each sum in
-//   one lane (each of the W lanes of a row group ends with g * kLoads / W of them), which exponentiates it;
-//   the weights go back to the group by shuffles for P·V. The running maximum is the warp's and moves only
-//   when a score exceeds it by 2^8. Warps are joined through shared memory, CTAs through the cluster's.
+// bf16 caches: every warp copies its own batches of 16 keys (8 KB) to shared memory, two ahead of the one that it
+// works on, with the warp-wide tensor instruction (mma.m16n8k16). Its 16
+// rows are the 8 query heads of a group twice, q as hi + lo bf16 terms (2^-16 of q is left out at most), so a
+// thread gets the two parts of a score in its own registers; the weights take the same places, hi rows and lo
+// rows, as the left operand of the value product. The inner index of a product may run over the elements in
+// any order, so K is read 16 bytes a lane as it lies and q laid out to match. 16 keys (8 KB) take about 130
+// instructions; multiplied element by element they took a thousand, and from registers, without the copies,
+// the loads in flight were too few.
 //
-// All fp32: q is not rounded, K and V as stored. What bounds it: the loads in flight, 16 warps of 4 KB (K and V
-// of 8 rows of 128) and their successors per SM.
+// fp32 caches: element by element; a row takes 16 or 32 lanes, every lane multiplies its elements for all
+// heads, one butterfly leaves each sum in one lane, which exponentiates it, and shuffles bring the weights back.
 #include "shared_decode.cuh"
 
 namespace sk {
 namespace shared {
 
-constexpr int kDirThreads = 256, kDirWarps = kDirThreads / 32, kMaxCluster = 8;
+constexpr int kMaxCluster = 8;
+constexpr int kDirThreads = 256, kDirWarps = kDirThreads / 32;  // fp32 caches
+constexpr int kMmaThreads = 128, kMmaWarps = kMmaThreads / 32;  // bf16 caches
 
 template <typename T>
 struct Pair;  // two neighbouring elements of a 16-byte load
-template <>
-struct Pair<__nv_bfloat16> {
-  static constexpr int E = 8;
-  static __device__ __forceinline__ float2 get(const uint4& v, int i) {
-    const uint32_t w = i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
-    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-  }
-  static __device__ __forceinline__ float rnd(float f) { return __bfloat162float(__float2bfloat16_rn(f)); }
-  static __device__ __forceinline__ __nv_bfloat16 st(float f) { return __float2bfloat16_rn(f); }
-};
 template <>
 struct Pair<float> {
   static constexpr int E = 4;
@@ -37,7 +33,6 @@ struct Pair<float> {
     return i == 0 ? make_float2(__uint_as_float(v.x), __uint_as_float(v.y))
                   : make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
   }
-  static __device__ __forceinline__ float rnd(float f) { return f; }
   static __device__ __forceinline__ float st(float f) { return f; }
 };
 
@@ -66,6 +61,349 @@ __device__ __forceinline__ float ld_remote(uint32_t addr) {
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
+// The end of both kernels: joins the warps' partials (ml, red: [warp][GP] and [warp][GP][HD]) and those of the
+// cluster's first `cluster` CTAs, the ones with rows, writes out, and adds the weights of the own rows [ja, jb), whose scores this CTA's warps wrote,
+// to the mass.
+template <int GP, int HD, int WARPS, int THREADS>
+__device__ __forceinline__ void finish(const Params& p, bool clustered, int cluster, int rank, int r, int kvh, int n, int ja, int jb,
+                                       const float2* ml_s, const float* red_s, float* o_s, float2* oml_s, float* M_s,
+                                       float* iL_s) {
+  constexpr int kThreads = THREADS;
+  const int g = p.g;
+  __syncthreads();
+  for (int x = threadIdx.x; x < g * HD; x += kThreads) {
+    const int h = x / HD;
+    float M = -INFINITY, L = 0.f, o = 0.f;
+#pragma unroll
+    for (int y = 0; y < WARPS; ++y) M = fmaxf(M, ml_s[y * GP + h].x);
+#pragma unroll
+    for (int y = 0; y < WARPS; ++y) {
+      const float a = ex2_approx(ml_s[y * GP + h].x - (M == -INFINITY ? 0.f : M));
+      L += a * ml_s[y * GP + h].y;
+      o += a * red_s[y * GP * HD + x];
+    }
+    o_s[x] = o;
+    if (x % HD == 0) oml_s[h] = make_float2(M, L);
+  }
+  __syncthreads();
+  if (clustered) {
+    cluster_arrive();
+    cluster_wait();
+  }
+  // out: each CTA of the cluster a run of the elements
+  const int total = g * HD, per = (total + cluster - 1) / cluster;
+  for (int x = rank * per + threadIdx.x; x < min(total, (rank + 1) * per); x += kThreads) {
+    const int h = x / HD;
+    float2 ml[kMaxCluster];
+    float part[kMaxCluster];
+#pragma unroll
+    for (int c = 0; c < kMaxCluster; ++c) {  // all in flight at once
+      ml[c] = make_float2(-INFINITY, 0.f);
+      part[c] = 0.f;
+      if (c < cluster) {
+        ml[c] = make_float2(ld_remote(mapa(&oml_s[h].x, c)), ld_remote(mapa(&oml_s[h].y, c)));
+        part[c] = ld_remote(mapa(o_s + x, c));
+      }
+    }
+    float M = ml[0].x, L = 0.f, o = 0.f;
+#pragma unroll
+    for (int c = 1; c < kMaxCluster; ++c) M = fmaxf(M, ml[c].x);
+#pragma unroll
+    for (int c = 0; c < kMaxCluster; ++c) {
+      const float a = c < cluster ? ex2_approx(ml[c].x - M) : 0.f;
+      L += a * ml[c].y;
+      o += a * part[c];
+    }
+    const long long at = r * p.out_stride + (long long)kvh * g * HD + x;
+    if (p.out_bf16)
+      reinterpret_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(o / L);
+    else
+      reinterpret_cast<float*>(p.out)[at] = o / L;
+  }
+  if (p.mass) {
+    if (threadIdx.x < g) {
+      const int h = threadIdx.x;
+      float2 ml[kMaxCluster];
+#pragma unroll
+      for (int c = 0; c < kMaxCluster; ++c)
+        ml[c] = c < cluster ? make_float2(ld_remote(mapa(&oml_s[h].x, c)), ld_remote(mapa(&oml_s[h].y, c)))
+                            : make_float2(-INFINITY, 0.f);
+      float M = ml[0].x, L = 0.f;
+#pragma unroll
+      for (int c = 1; c < kMaxCluster; ++c) M = fmaxf(M, ml[c].x);
+#pragma unroll
+      for (int c = 0; c < kMaxCluster; ++c) L += c < cluster ? ex2_approx(ml[c].x - M) * ml[c].y : 0.f;
+      M_s[h] = M;
+      iL_s[h] = 1.f / L;
+    }
+    __syncthreads();
+    float* mass = p.mass + r * p.mass_request_stride + kvh * p.mass_head_stride;
+    const float* sc = p.sc + ((long long)r * p.nq + kvh * g) * p.sc_stride;
+    constexpr int kAtOnce = 4;  // rows per thread whose loads are in flight together
+    for (int j0 = ja + threadIdx.x; j0 < jb; j0 += kThreads * kAtOnce) {
+      float sum[kAtOnce], before[kAtOnce];
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int j = j0 + i * kThreads;
+        before[i] = j < min(n, jb) ? mass[j] : 0.f;  // the new row starts from nothing
+        sum[i] = 0.f;
+      }
+      for (int h = 0; h < g; ++h) {
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+          const int j = j0 + i * kThreads;
+          if (j < jb) sum[i] += ex2_approx(__ldcg(sc + h * p.sc_stride + j) - M_s[h]) * iL_s[h];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int j = j0 + i * kThreads;
+        if (j < jb) mass[j] = before[i] + sum[i];
+      }
+    }
+  }
+  if (clustered) {  // no CTA leaves while another reads its partial
+    cluster_arrive();
+    cluster_wait();
+  }
+}
+
+// ---- bf16 caches -----------------------------------------------------------------------------------
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// x's two bf16 terms, a pair at a time
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+  hi = pack2(a, b);
+  lo = pack2(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u));
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&d)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+               : "r"(addr)
+               : "memory");
+}
+
+// 16 bytes to shared memory; `keep` false writes zeros and reads nothing.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool keep) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(keep ? 16 : 0) : "memory");
+}
+
+template <int HD>
+struct MmaSmem {
+  static constexpr int kRows = 16;                // keys of a batch
+  // Batches in a warp's ring, CTAs per SM (measured, graph: 16 slots of 128 18.1 us with 3 and 2 against 20.0
+  // with 2 and 3; 45 requests of 4 heads of 64 21.9 us with 4 and 3 against 29.1 with 6 and 2).
+  static constexpr int NST = HD == 128 ? 3 : 4, kPerSm = HD == 128 ? 2 : 3;
+  static constexpr int PITCH = HD * 2 + 16;       // bytes: an odd number of 16-byte units, no bank conflicts
+  static constexpr int HALF = kRows * PITCH, SLOT = 2 * HALF;  // K, V
+  static constexpr int OFF_Q = kMmaWarps * NST * SLOT;           // [hi, lo][8 rows][PITCH]
+  static constexpr int OFF_NEW = OFF_Q + 2 * kMaxGroup * PITCH;  // the new token's k and v
+  static constexpr int BYTES = OFF_NEW + 2 * HD * 2;
+  // after the last batch the rings hold the warps' outputs and the CTA's
+  static constexpr int OFF_RED = 0, OFF_O = kMmaWarps * kMaxGroup * HD * 4;
+  static_assert(OFF_O + kMaxGroup * HD * 4 <= OFF_Q, "the outputs fit the rings");
+};
+
+template <int HD>
+__global__ void __launch_bounds__(kMmaThreads, MmaSmem<HD>::kPerSm) direct_mma_kernel(const Params p, int cluster) {
+  using S = MmaSmem<HD>;
+  constexpr int GP = kMaxGroup, EL = HD / 32, NST = S::NST, kRows = S::kRows;
+  constexpr int NP = HD / 32;  // 16-byte pieces of a K row per lane: elements 32 i + 8 (lane % 4) ...
+  constexpr int U = HD / 8, RPI = 32 / U;  // 16-byte units of a row, rows per instruction of a warp's copy
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float2 ml_s[kMmaWarps][GP], oml_s[GP];
+  __shared__ float M_s[GP], iL_s[GP];
+  uint8_t* new_s = smem + S::OFF_NEW;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = lane & 3, row = lane >> 2;
+  const int item = blockIdx.x / cluster, rank = blockIdx.x % cluster;  // clusters are consecutive CTAs
+  const int r = item / p.nkv, kvh = item - r * p.nkv, g = p.g;
+
+  griddep_wait();
+  griddep_launch_dependents();
+  const long long pos64 = p.pos[r], own64 = p.rows ? p.rows[r] : pos64 - p.P;
+  // rows 0 .. g-1: q; g: k; g + 1: v
+  const long long qkv_at = r * p.qkv_stride;
+  auto source = [&](int x) { return qkv_at + (long long)(x < g ? kvh * g + x : x == g ? p.nq + kvh : p.nq + p.nkv + kvh) * HD; };
+  RawRow<HD> raw[1];
+  if (w < g + 2) raw[0].load(p.qkv, source(w), p.qkv_bf16);
+  const bool idle = pos64 < 0, bad = !idle && (pos64 >= p.rope_len || own64 < 0 || own64 >= p.max_len);
+  if (idle || bad) {  // uniform over the cluster
+    if (bad && rank == 0 && kvh == 0 && threadIdx.x == 0) set_dev_error(p.err, SK_DEVERR_POS_RANGE);
+    return;
+  }
+  const int n = (int)own64, pos = (int)pos64;
+  const long long own_at = r * p.request_stride + kvh * p.head_stride, prefix_at = kvh * p.prefix_head_stride;
+  // Batches of the prefix, then of the own rows with the new one (own row n); a run of them per CTA of the
+  // cluster, dealt out to its warps in turn.
+  const int nbp = (p.P + kRows - 1) / kRows, nb = nbp + n / kRows + 1;
+  const int run = (nb + cluster - 1) / cluster, b0 = rank * run, b1 = min(nb, b0 + run);
+  if (b0 >= nb) return;  // the cluster's barriers wait for threads that have not exited only
+  const int active = (nb + run - 1) / run;
+  const uint32_t ring = smem_u32(smem) + w * NST * S::SLOT;
+  // Batch b into slot `slot` of this warp's ring; rows past the end become zeros (their weight is zero, and
+  // zero it stays whatever the cache holds there). One group of copies per batch, an empty one past the last.
+  auto fetch = [&](int b, int slot) __attribute__((always_inline)) {
+    if (b < b1) {
+      const bool own = b >= nbp;
+      const int j0 = (own ? b - nbp : b) * kRows, valid = (own ? n : p.P) - j0, x = lane / U, u = lane % U;
+      const long long pitch = own ? p.row_stride : p.prefix_row_stride;
+      const long long at = (own ? own_at : prefix_at) + (j0 + x) * pitch + u * 8;
+      const __nv_bfloat16* k = reinterpret_cast<const __nv_bfloat16*>(own ? p.Kc : p.Kp) + at;
+      const __nv_bfloat16* v = reinterpret_cast<const __nv_bfloat16*>(own ? p.Vc : p.Vp) + at;
+      const uint32_t dst = ring + slot * S::SLOT + x * S::PITCH + u * 16;
+#pragma unroll
+      for (int i = 0; i < kRows; i += RPI) {
+        const bool in = i + x < valid;
+        cp_async16(dst + i * S::PITCH, in ? k + i * pitch : k - x * pitch, in);
+        cp_async16(dst + S::HALF + i * S::PITCH, in ? v + i * pitch : v - x * pitch, in);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < NST - 1; ++i) fetch(b0 + w + i * kMmaWarps, i);
+
+  // q, and the new token's k and v
+  for (int x = w; x < GP; x += kMmaWarps)  // the rows of heads that are not there
+    if (x >= g && lane < U) {
+      *reinterpret_cast<uint4*>(smem + S::OFF_Q + x * S::PITCH + lane * 16) = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(smem + S::OFF_Q + (GP + x) * S::PITCH + lane * 16) = make_uint4(0, 0, 0, 0);
+    }
+  for (int x = w; x < g + 2; x += kMmaWarps) {
+    if (x != w) raw[0].load(p.qkv, source(x), p.qkv_bf16);
+    float y[1][EL];
+    if (x <= g) {
+      const int ps[1] = {pos};
+      norm_rotate_rows<HD, 1>(y, raw, p.qkv_bf16, ps, x < g ? p.qn : p.kn, p.rope, p.eps);
+    } else {
+      raw[0].values(p.qkv_bf16, y[0]);
+    }
+    if (x < g) {
+#pragma unroll
+      for (int e = 0; e < EL; e += 2) {
+        uint32_t hi, lo;
+        split2(y[0][e] * p.q_scale, y[0][e + 1] * p.q_scale, hi, lo);
+        *reinterpret_cast<uint32_t*>(smem + S::OFF_Q + x * S::PITCH + (lane * EL + e) * 2) = hi;
+        *reinterpret_cast<uint32_t*>(smem + S::OFF_Q + (GP + x) * S::PITCH + (lane * EL + e) * 2) = lo;
+      }
+    } else {
+      __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(x == g ? p.Kc : p.Vc) + own_at + n * p.row_stride + lane * EL;
+#pragma unroll
+      for (int e = 0; e < EL; e += 2) {
+        const uint32_t two = pack2(y[0][e], y[0][e + 1]);
+        *reinterpret_cast<uint32_t*>(new_s + ((x - g) * HD + lane * EL + e) * 2) = two;
+        if (rank == 0) *reinterpret_cast<uint32_t*>(dst + e) = two;
+      }
+    }
+  }
+  __syncthreads();
+
+  float m = -INFINITY, l = 0.f;  // of head `row`, the same in its four lanes / this lane's part
+  float o[HD / 8][4];            // head `row`: elements 8 t + 2c, + 1 by hi weights, then by lo
+#pragma unroll
+  for (int t = 0; t < HD / 8; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
+  float* sc = p.mass && row < g ? p.sc + ((long long)r * p.nq + kvh * g + row) * p.sc_stride : nullptr;
+  const uint8_t* q_at = smem + S::OFF_Q + row * S::PITCH + 16 * c;
+  // ldmatrix: lane x gives the row of matrix x / 8: keys x % 8 (+ 8 for the odd ones), 8 elements on for 2 and 3
+  const uint32_t v_at = S::HALF + (lane & 15) * S::PITCH + (lane >> 4) * 16;
+
+  int slot = 0;
+#pragma unroll 1
+  for (int b = b0 + w; b < b1; b += kMmaWarps) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(NST - 2) : "memory");
+    __syncwarp();  // this batch has landed for every lane, and every lane is past the one whose slot is next
+    fetch(b + (NST - 1) * kMmaWarps, slot == 0 ? NST - 1 : slot - 1);
+    uint8_t* at = smem + w * NST * S::SLOT + slot * S::SLOT;
+    const bool own = b >= nbp;
+    const int j0 = (own ? b - nbp : b) * kRows, valid = own ? n + 1 - j0 : p.P - j0;  // rows, if fewer than 16
+    if (b == nb - 1) {  // the new row in its place
+      uint8_t* dst = at + (n - j0) * S::PITCH;
+      for (int x = lane; x < 2 * U; x += 32)
+        *reinterpret_cast<uint4*>(dst + (x / U) * S::HALF + (x % U) * 16) = *reinterpret_cast<const uint4*>(new_s + x * 16);
+      __syncwarp();
+    }
+    const uint8_t* k_at = at + row * S::PITCH + 16 * c;
+    float s[2][4], s2[2][4];  // two chains of products each
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[u][e] = s2[u][e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const uint4 hi = *reinterpret_cast<const uint4*>(q_at + 64 * i);
+      const uint4 lo = *reinterpret_cast<const uint4*>(q_at + GP * S::PITCH + 64 * i);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint4 k = *reinterpret_cast<const uint4*>(k_at + 8 * u * S::PITCH + 64 * i);
+        mma_bf16(s[u], hi.x, lo.x, hi.y, lo.y, k.x, k.y);
+        mma_bf16(s2[u], hi.z, lo.z, hi.w, lo.w, k.z, k.w);
+      }
+    }
+    bool over = false;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int j = 8 * u + 2 * c + e;
+        s[u][e] = j < valid ? (s[u][e] + s2[u][e]) + (s[u][2 + e] + s2[u][2 + e]) : -INFINITY;
+        over |= row < g && s[u][e] > m + 8.0f;
+        if (sc && own && j < valid) sc[j0 + j] = s[u][e];
+      }
+    if (__any_sync(0xffffffffu, over)) {
+      float t = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
+      t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+      t = fmaxf(fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2)), m);
+      const float a = t == -INFINITY ? 1.f : ex2_approx(m - t);
+      m = t;
+      l *= a;
+#pragma unroll
+      for (int x = 0; x < HD / 8; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[x][e] *= a;
+    }
+    const float use = m == -INFINITY ? 0.f : m;
+    uint32_t a[4];  // left operand: hi rows (keys of u = 0), lo rows, hi rows (u = 1), lo rows
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const float x = ex2_approx(s[u][0] - use), y = ex2_approx(s[u][1] - use);
+      l += x + y;
+      split2(x, y, a[2 * u], a[2 * u + 1]);
+    }
+#pragma unroll
+    for (int t = 0; t < HD / 8; t += 2) {
+      uint32_t vb[4];
+      ldmatrix_x4_trans(vb, ring + slot * S::SLOT + v_at + t * 16);
+      mma_bf16(o[t], a[0], a[1], a[2], a[3], vb[0], vb[1]);
+      mma_bf16(o[t + 1], a[0], a[1], a[2], a[3], vb[2], vb[3]);
+    }
+    slot = slot == NST - 1 ? 0 : slot + 1;
+  }
+
+  l += __shfl_xor_sync(0xffffffffu, l, 1);
+  l += __shfl_xor_sync(0xffffffffu, l, 2);
+  if (c == 0) ml_s[w][row] = make_float2(m, l);
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();  // every batch read: the rings take the outputs
+  if (row < g) {
+#pragma unroll
+    for (int t = 0; t < HD / 8; ++t)
+      *reinterpret_cast<float2*>(smem + S::OFF_RED + (((w * GP + row) * HD) + 8 * t + 2 * c) * 4) =
+          make_float2(o[t][0] + o[t][2], o[t][1] + o[t][3]);
+  }
+  finish<GP, HD, kMmaWarps, kMmaThreads>(p, cluster > 1, active, rank, r, kvh, n, max(0, b0 - nbp) * kRows, min(n + 1, (b1 - nbp) * kRows),
+                                         &ml_s[0][0], reinterpret_cast<const float*>(smem + S::OFF_RED),
+                                         reinterpret_cast<float*>(smem + S::OFF_O), oml_s, M_s, iL_s);
+}
+
+// ---- fp32 caches -----------------------------------------------------------------------------------
 // Lanes per row, rows per load, loads per batch.
 template <typename T, int HD, int GP>
 struct DirectCfg {
@@ -75,20 +413,23 @@ struct DirectCfg {
   static constexpr int NV = kLoads * GP;         // sums per row group
   static constexpr int VK = NV > W ? NV / W : 1; // of which a lane keeps this many
   static constexpr int REP = NV < W ? W / NV : 1;  // lanes that hold the same one
-  static constexpr bool kAhead = GP <= 2;        // the next batch in registers
+  static constexpr bool kAhead = GP <= 2;  // the next batch in registers
+  static constexpr bool kQRegs = GP <= 2;  // q in registers, else read from shared memory
+  static constexpr int kPerSm = GP <= 4 ? 2 : 1;
 };
 
 template <typename T, int HD, int GP>
-__global__ void __launch_bounds__(kDirThreads, GP <= 4 ? 2 : 1) direct_kernel(const Params p, int cluster) {
+__global__ void __launch_bounds__(kDirThreads, DirectCfg<T, HD, GP>::kPerSm) direct_kernel(const Params p, int cluster) {
   using C = DirectCfg<T, HD, GP>;
   constexpr int E = C::E, W = C::W, RPL = C::RPL, NL = C::kLoads, NV = C::NV, VK = C::VK, REP = C::REP, EL = HD / 32;
+  constexpr int kRows = C::kRows;
   __shared__ __align__(16) float q_s[GP][HD];
-  __shared__ __align__(16) float kv_s[2][HD];              // the new token's k and v as the cache holds them
+  __shared__ __align__(16) T new_s[2][HD];                 // the new token's k and v as the cache holds them
   __shared__ __align__(16) float red_s[kDirWarps][GP][HD];
   __shared__ float2 ml_s[kDirWarps][GP];
   __shared__ __align__(16) float o_s[GP][HD];              // the CTA's partial (read by the cluster)
   __shared__ float2 oml_s[GP];
-  __shared__ float snew_s[GP], M_s[GP], iL_s[GP];
+  __shared__ float M_s[GP], iL_s[GP];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, sub = lane % W, grp = lane / W;
   const int item = blockIdx.x / cluster, rank = blockIdx.x % cluster;  // clusters are consecutive CTAs
   const int r = item / p.nkv, kvh = item - r * p.nkv, g = p.g;
@@ -97,38 +438,41 @@ __global__ void __launch_bounds__(kDirThreads, GP <= 4 ? 2 : 1) direct_kernel(co
   griddep_launch_dependents();
   const long long pos64 = p.pos[r], own64 = p.rows ? p.rows[r] : pos64 - p.P;
   RawRow<HD> raw[1];  // warps 0 .. g-1: q rows; g: k; g + 1: v (several per warp where g + 2 > 8)
-  raw[0].load(p.qkv, r * p.qkv_stride + (long long)(w < g ? kvh * g + w : w == g ? p.nq + kvh : p.nq + p.nkv + kvh) * HD,
-              p.qkv_bf16);
+  if (w < g + 2)
+    raw[0].load(p.qkv, r * p.qkv_stride + (long long)(w < g ? kvh * g + w : w == g ? p.nq + kvh : p.nq + p.nkv + kvh) * HD,
+                p.qkv_bf16);
   const bool idle = pos64 < 0, bad = !idle && (pos64 >= p.rope_len || own64 < 0 || own64 >= p.max_len);
   if (idle || bad) {  // uniform over the cluster
     if (bad && rank == 0 && kvh == 0 && threadIdx.x == 0) set_dev_error(p.err, SK_DEVERR_POS_RANGE);
     return;
   }
-  const int n = (int)own64, P = p.P, N = P + n;
-  const int pos = (int)pos64;
-  const char* Kp = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.Kp) + kvh * p.prefix_head_stride) + sub * 16;
-  const char* Vp = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.Vp) + kvh * p.prefix_head_stride) + sub * 16;
+  const int n = (int)own64, pos = (int)pos64;
   const long long own_at = r * p.request_stride + kvh * p.head_stride;
-  const char* Kc = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.Kc) + own_at) + sub * 16;
-  const char* Vc = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.Vc) + own_at) + sub * 16;
-  const int batches = (N + C::kRows - 1) / C::kRows, stride = cluster * kDirWarps;
+  // Batches of the prefix, then of the own rows with the new one (own row n, taken from shared memory); a run
+  // of them per CTA of the cluster, dealt out to its warps in turn.
+  const int nbp = (p.P + kRows - 1) / kRows, nb = nbp + n / kRows + 1;
+  const int run = (nb + cluster - 1) / cluster, b1 = min(nb, (rank + 1) * run), b0 = rank * run + w;
+  if (rank * run >= nb) return;  // the cluster's barriers wait for threads that have not exited only
+  const int active = (nb + run - 1) / run;
 
   uint4 k[NL], v[NL];
-  auto load = [&](int b, uint4 (&kk)[NL], uint4 (&vv)[NL]) {
+  auto load = [&](int b, uint4 (&kk)[NL], uint4 (&vv)[NL]) __attribute__((always_inline)) {
+    const bool own = b >= nbp;
+    const int j0 = (own ? b - nbp : b) * kRows, valid = (own ? n : p.P) - j0;
+    const long long pitch = own ? p.row_stride : p.prefix_row_stride;
+    const long long at = (own ? own_at : kvh * p.prefix_head_stride) + (j0 + grp) * pitch + sub * E;
+    const T* kp = reinterpret_cast<const T*>(own ? p.Kc : p.Kp) + at;
+    const T* vp = reinterpret_cast<const T*>(own ? p.Vc : p.Vp) + at;
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      const int j = b * C::kRows + i * RPL + grp;
-      const bool own = j >= P;
-      const long long at = (own ? (j - P) * p.row_stride : j * p.prefix_row_stride) * (long long)sizeof(T);
       kk[i] = vv[i] = make_uint4(0, 0, 0, 0);
-      if (j < N) {
-        kk[i] = ld_stream((own ? Kc : Kp) + at);
-        vv[i] = ld_stream((own ? Vc : Vp) + at);
+      if (i * RPL + grp < valid) {
+        kk[i] = ld_stream(kp + i * RPL * pitch);
+        vv[i] = ld_stream(vp + i * RPL * pitch);
       }
     }
   };
-  const int b0 = rank * kDirWarps + w;
-  if (b0 < batches) load(b0, k, v);
+  if (b0 < b1) load(b0, k, v);
 
   // q, and the new token's k and v
   for (int x = w; x < g + 2; x += kDirWarps) {
@@ -139,19 +483,21 @@ __global__ void __launch_bounds__(kDirThreads, GP <= 4 ? 2 : 1) direct_kernel(co
     if (x <= g) {
       const int ps[1] = {pos};
       norm_rotate_rows<HD, 1>(y, raw, p.qkv_bf16, ps, x < g ? p.qn : p.kn, p.rope, p.eps);
-#pragma unroll
-      for (int e = 0; e < EL; ++e) y[0][e] = x < g ? y[0][e] * p.q_scale : Pair<T>::rnd(y[0][e]);
-      store_vec<EL>((x < g ? q_s[x] : kv_s[0]) + lane * EL, y[0]);
     } else {
       raw[0].values(p.qkv_bf16, y[0]);
-#pragma unroll
-      for (int e = 0; e < EL; ++e) y[0][e] = Pair<T>::rnd(y[0][e]);
-      store_vec<EL>(kv_s[1] + lane * EL, y[0]);
     }
-    if (rank == 0 && x >= g) {  // appended as own row n
+    if (x < g) {
+#pragma unroll
+      for (int e = 0; e < EL; ++e) y[0][e] *= p.q_scale;
+      store_vec<EL>(q_s[x] + lane * EL, y[0]);
+    } else {
       T* dst = reinterpret_cast<T*>(x == g ? p.Kc : p.Vc) + own_at + n * p.row_stride + lane * EL;
 #pragma unroll
-      for (int e = 0; e < EL; ++e) dst[e] = Pair<T>::st(y[0][e]);
+      for (int e = 0; e < EL; ++e) {
+        const T t = Pair<T>::st(y[0][e]);
+        new_s[x - g][lane * EL + e] = t;
+        if (rank == 0) dst[e] = t;
+      }
     }
   }
   __syncthreads();
@@ -160,41 +506,31 @@ __global__ void __launch_bounds__(kDirThreads, GP <= 4 ? 2 : 1) direct_kernel(co
   float2 acc[GP][E / 2] = {};
 #pragma unroll
   for (int h = 0; h < GP; ++h) m[h] = -INFINITY;
-  float2 q[C::kAhead ? GP : 1][E / 2];
-  if (C::kAhead) {
+  float2 q[C::kQRegs ? GP : 1][E / 2];
+  if (C::kQRegs) {
 #pragma unroll
     for (int h = 0; h < GP; ++h)
 #pragma unroll
       for (int e = 0; e < E / 2; ++e)
-        q[C::kAhead ? h : 0][e] = h < g ? *reinterpret_cast<const float2*>(q_s[h] + sub * E + 2 * e) : make_float2(0.f, 0.f);
+        q[C::kQRegs ? h : 0][e] = h < g ? *reinterpret_cast<const float2*>(q_s[h] + sub * E + 2 * e) : make_float2(0.f, 0.f);
   }
   // value x = row slot * GP + head of a row group is kept by the lane (or the REP lanes) that sub / REP = x / VK
   const int x0 = sub / REP * VK;
-  // the new token is the first partial of warp 0 of the cluster's first CTA, its weight 1 in the sum that
-  // row slot 0 has for the head
-  if (rank == 0 && w == 0) {
+
+  for (int b = b0; b < b1; b += kDirWarps) {
+    uint4 kn[NL], vn[NL];
+    if (C::kAhead && b + kDirWarps < b1) load(b + kDirWarps, kn, vn);
+    const bool own = b >= nbp;
+    const int j0 = (own ? b - nbp : b) * kRows, valid = own ? n + 1 - j0 : p.P - j0;  // rows of the batch, if fewer than kRows
+    if (b == nb - 1) {  // by selects, which keep k and v in registers
+      const uint4 k1 = *reinterpret_cast<const uint4*>(new_s[0] + sub * E), v1 = *reinterpret_cast<const uint4*>(new_s[1] + sub * E);
 #pragma unroll
-    for (int h = 0; h < GP; ++h) {
-      if (h >= g) break;
-      float d = 0.f;
-#pragma unroll
-      for (int e = 0; e < EL; ++e) d += q_s[h][lane * EL + e] * kv_s[0][lane * EL + e];
-      m[h] = warp_sum32(d);
-      if (lane == 0) snew_s[h] = m[h];
-      if (grp == 0) {
-#pragma unroll
-        for (int e = 0; e < E / 2; ++e) acc[h][e] = *reinterpret_cast<const float2*>(kv_s[1] + sub * E + 2 * e);
+      for (int i = 0; i < NL; ++i) {
+        const bool it = i * RPL + grp == n - j0;
+        k[i] = make_uint4(it ? k1.x : k[i].x, it ? k1.y : k[i].y, it ? k1.z : k[i].z, it ? k1.w : k[i].w);
+        v[i] = make_uint4(it ? v1.x : v[i].x, it ? v1.y : v[i].y, it ? v1.z : v[i].z, it ? v1.w : v[i].w);
       }
     }
-    if (grp == 0 && sub % REP == 0) {
-#pragma unroll
-      for (int c = 0; c < VK; ++c) l[c] = x0 + c < g ? 1.f : 0.f;
-    }
-  }
-
-  for (int b = b0; b < batches; b += stride) {
-    uint4 kn[NL], vn[NL];
-    if (C::kAhead && b + stride < batches) load(b + stride, kn, vn);
     float s[NV];
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
@@ -203,7 +539,7 @@ __global__ void __launch_bounds__(kDirThreads, GP <= 4 ? 2 : 1) direct_kernel(co
         float2 d = make_float2(0.f, 0.f);
 #pragma unroll
         for (int e = 0; e < E / 2; ++e) {
-          const float2 qq = C::kAhead ? q[C::kAhead ? h : 0][e] : *reinterpret_cast<const float2*>(q_s[h] + sub * E + 2 * e);
+          const float2 qq = C::kQRegs ? q[C::kQRegs ? h : 0][e] : *reinterpret_cast<const float2*>(q_s[h] + sub * E + 2 * e);
           d = __ffma2_rn(Pair<T>::get(k[i], e), qq, d);
         }
         s[i * GP + h] = d.x + d.y;
@@ -227,14 +563,14 @@ __global__ void __launch_bounds__(kDirThreads, GP <= 4 ? 2 : 1) direct_kernel(co
     float mo[VK];
 #pragma unroll
     for (int c = 0; c < VK; ++c) {
-      const int x = x0 + c, h = x % GP, j = b * C::kRows + x / GP * RPL + grp;
-      if (j >= N || h >= g) s[c] = -INFINITY;
+      const int x = x0 + c, h = x % GP, j = x / GP * RPL + grp;
+      if (j >= valid || h >= g) s[c] = -INFINITY;
       mo[c] = m[0];
 #pragma unroll
       for (int y = 1; y < GP; ++y) mo[c] = y == h ? m[y] : mo[c];
       over |= s[c] > mo[c] + 8.0f;
-      if (p.mass && j >= P && j < N && h < g && (REP == 1 || sub % REP == 0))
-        p.sc[((long long)r * p.nq + kvh * g + h) * p.sc_stride + (j - P)] = s[c];
+      if (p.mass && own && j < valid && h < g && (REP == 1 || sub % REP == 0))
+        p.sc[((long long)r * p.nq + kvh * g + h) * p.sc_stride + j0 + j] = s[c];
     }
     if (__any_sync(0xffffffffu, over)) {
       float a[GP];
@@ -278,8 +614,8 @@ __global__ void __launch_bounds__(kDirThreads, GP <= 4 ? 2 : 1) direct_kernel(co
     if (C::kAhead) {
 #pragma unroll
       for (int i = 0; i < NL; ++i) k[i] = kn[i], v[i] = vn[i];
-    } else if (b + stride < batches) {
-      load(b + stride, k, v);
+    } else if (b + kDirWarps < b1) {
+      load(b + kDirWarps, k, v);
     }
   }
 
@@ -297,110 +633,25 @@ __global__ void __launch_bounds__(kDirThreads, GP <= 4 ? 2 : 1) direct_kernel(co
         acc[h][e].x += __shfl_xor_sync(0xffffffffu, acc[h][e].x, o);
         acc[h][e].y += __shfl_xor_sync(0xffffffffu, acc[h][e].y, o);
       }
-    __syncwarp();
     if (lane == 0) ml_s[w][h] = make_float2(m[h], t);
     if (grp == 0) {
 #pragma unroll
       for (int e = 0; e < E / 2; ++e) *reinterpret_cast<float2*>(red_s[w][h] + sub * E + 2 * e) = acc[h][e];
     }
   }
-  __syncthreads();
-  // the CTA's
-  for (int x = threadIdx.x; x < g * HD; x += kDirThreads) {
-    const int h = x / HD, d = x % HD;
-    float M = -INFINITY, L = 0.f, o = 0.f;
-#pragma unroll
-    for (int y = 0; y < kDirWarps; ++y) M = fmaxf(M, ml_s[y][h].x);
-#pragma unroll
-    for (int y = 0; y < kDirWarps; ++y) {
-      const float a = ex2_approx(ml_s[y][h].x - (M == -INFINITY ? 0.f : M));
-      L += a * ml_s[y][h].y;
-      o += a * red_s[y][h][d];
-    }
-    o_s[h][d] = o;
-    if (d == 0) oml_s[h] = make_float2(M, L);
-  }
-  __syncthreads();
-  if (cluster > 1) {
-    cluster_arrive();
-    cluster_wait();
-  }
-  // out: element x by CTA x % cluster ... each CTA a run of them
-  const int total = g * HD, per = (total + cluster - 1) / cluster;
-  for (int x = rank * per + threadIdx.x; x < min(total, (rank + 1) * per); x += kDirThreads) {
-    const int h = x / HD, d = x % HD;
-    float2 ml[kMaxCluster];
-    float part[kMaxCluster];
-#pragma unroll
-    for (int c = 0; c < kMaxCluster; ++c) {  // all in flight at once
-      ml[c] = make_float2(-INFINITY, 0.f);
-      part[c] = 0.f;
-      if (c < cluster) {
-        ml[c] = make_float2(ld_remote(mapa(&oml_s[h].x, c)), ld_remote(mapa(&oml_s[h].y, c)));
-        part[c] = ld_remote(mapa(&o_s[h][d], c));
-      }
-    }
-    float M = ml[0].x, L = 0.f, o = 0.f;
-#pragma unroll
-    for (int c = 1; c < kMaxCluster; ++c) M = fmaxf(M, ml[c].x);
-#pragma unroll
-    for (int c = 0; c < kMaxCluster; ++c) {
-      const float a = c < cluster ? ex2_approx(ml[c].x - M) : 0.f;
-      L += a * ml[c].y;
-      o += a * part[c];
-    }
-    const long long at = r * p.out_stride + (long long)kvh * g * HD + x;
-    if (p.out_bf16)
-      reinterpret_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(o / L);
-    else
-      reinterpret_cast<float*>(p.out)[at] = o / L;
-  }
-  if (p.mass) {
-    if (threadIdx.x < g) {
-      const int h = threadIdx.x;
-      float2 ml[kMaxCluster];
-#pragma unroll
-      for (int c = 0; c < kMaxCluster; ++c)
-        ml[c] = c < cluster ? make_float2(ld_remote(mapa(&oml_s[h].x, c)), ld_remote(mapa(&oml_s[h].y, c)))
-                            : make_float2(-INFINITY, 0.f);
-      float M = ml[0].x, L = 0.f;
-#pragma unroll
-      for (int c = 1; c < kMaxCluster; ++c) M = fmaxf(M, ml[c].x);
-#pragma unroll
-      for (int c = 0; c < kMaxCluster; ++c) L += c < cluster ? ex2_approx(ml[c].x - M) * ml[c].y : 0.f;
-      M_s[h] = M;
-      iL_s[h] = 1.f / L;
-    }
-    __syncthreads();
-    // the rows whose scores this CTA's warps have written
-    float* mass = p.mass + r * p.mass_request_stride + kvh * p.mass_head_stride;
-    const float* sc = p.sc + ((long long)r * p.nq + kvh * g) * p.sc_stride;
-    for (int b = b0; b < batches; b += stride) {
-      const int j = b * C::kRows + lane - P;
-      if (lane < C::kRows && j >= 0 && j < n) {
-        float a = 0.f;
-        for (int h = 0; h < g; ++h) a += ex2_approx(__ldcg(sc + h * p.sc_stride + j) - M_s[h]) * iL_s[h];
-        mass[j] += a;
-      }
-    }
-    if (rank == 0 && threadIdx.x == 0) {
-      float a = 0.f;
-      for (int h = 0; h < g; ++h) a += ex2_approx(snew_s[h] - M_s[h]) * iL_s[h];
-      mass[n] = a;
-    }
-  }
-  if (cluster > 1) {  // no CTA leaves while another reads its partial
-    cluster_arrive();
-    cluster_wait();
-  }
+  finish<GP, HD, kDirWarps, kDirThreads>(p, cluster > 1, active, rank, r, kvh, n, max(0, rank * run - nbp) * kRows, min(n + 1, (b1 - nbp) * kRows),
+                            &ml_s[0][0], &red_s[0][0][0], &o_s[0][0], oml_s, M_s, iL_s);
 }
 
 // ---- host -----------------------------------------------------------------------------------------
-template <typename T, int HD, int GP>
-static int launch(const Params& p, int cluster, cudaStream_t st) {
+static int launch(void (*kernel)(const Params, int), int threads, int smem, const Params& p, int cluster, cudaStream_t st) {
+  if (smem > 48 * 1024 &&
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return SK_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
+  cfg.dynamicSmemBytes = (size_t)smem;
   cfg.gridDim = dim3((unsigned)(p.R * p.nkv * cluster));
-  cfg.blockDim = dim3(kDirThreads);
+  cfg.blockDim = dim3((unsigned)threads);
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -410,26 +661,28 @@ static int launch(const Params& p, int cluster, cudaStream_t st) {
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, direct_kernel<T, HD, GP>, p, cluster) == cudaSuccess ? SK_OK : SK_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, kernel, p, cluster) == cudaSuccess ? SK_OK : SK_ERR_CUDA;
 }
-template <typename T, int HD>
-static int launch_group(const Params& p, int cluster, cudaStream_t st) {
-  if (p.g == 1) return launch<T, HD, 1>(p, cluster, st);
-  if (p.g == 2) return launch<T, HD, 2>(p, cluster, st);
-  if (p.g <= 4) return launch<T, HD, 4>(p, cluster, st);
-  return launch<T, HD, 8>(p, cluster, st);
+template <int HD>
+static void (*f32_kernel(int g))(const Params, int) {
+  return g == 1   ? direct_kernel<float, HD, 1>
+         : g == 2 ? direct_kernel<float, HD, 2>
+         : g <= 4 ? direct_kernel<float, HD, 4> : direct_kernel<float, HD, 8>;
 }
 
-int launch_direct(const Params& p, int hd, int cache_dtype, cudaStream_t st) {
-  // CTAs per (request, head): as many as keep the grid within two CTAs per SM and give every warp a batch
-  const int rows = cache_dtype == SK_BF16 ? (hd == 128 ? 8 : 16) : (hd == 128 ? 4 : 8);
+int launch_direct(const Params& p, int hd, cudaStream_t st) {
+  // CTAs per (request, head): up to 8, while the SMs hold them all and every warp gets a batch. (Runs of a fixed
+  // length, so that long requests get more CTAs than short ones, took longer: 19 to 29 us for 16 slots of 1 to
+  // 1404 rows against 18, clusters of which most CTAs leave at once being slow to start.)
+  const int per = p.f32 ? (hd == 128 ? 4 : 8) : 16, warps = p.f32 ? kDirWarps : kMmaWarps;
+  const int slots = 148 * (p.f32 ? 2 : hd == 128 ? MmaSmem<128>::kPerSm : MmaSmem<64>::kPerSm);
+  const long long heads = (long long)p.R * p.nkv, most = (p.P + per - 1) / per + p.max_len / per + 1;  // batches
   int cluster = 1;
-  while (cluster < kMaxCluster && (long long)p.R * p.nkv * cluster * 2 <= 296 &&
-         (long long)(p.P + p.max_len) > (long long)cluster * kDirWarps * rows)
-    cluster *= 2;
-  if (cache_dtype == SK_BF16)
-    return hd == 128 ? launch_group<__nv_bfloat16, 128>(p, cluster, st) : launch_group<__nv_bfloat16, 64>(p, cluster, st);
-  return hd == 128 ? launch_group<float, 128>(p, cluster, st) : launch_group<float, 64>(p, cluster, st);
+  while (cluster < kMaxCluster && heads * cluster * 2 <= slots && most > cluster * warps) cluster *= 2;
+  if (p.f32)
+    return launch(hd == 128 ? f32_kernel<128>(p.g) : f32_kernel<64>(p.g), kDirThreads, 0, p, cluster, st);
+  return hd == 128 ? launch(direct_mma_kernel<128>, kMmaThreads, MmaSmem<128>::BYTES, p, cluster, st)
+                   : launch(direct_mma_kernel<64>, kMmaThreads, MmaSmem<64>::BYTES, p, cluster, st);
 }
 
 }  // namespace shared

@@ -49,22 +49,6 @@ __device__ __forceinline__ void setmaxnreg_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-// mbar_wait in as few instructions as it takes: the kernel has some twenty waits, and its start is bound by
-// instruction fetches.
-__device__ __forceinline__ bool wait_on(uint64_t* bar, int phase, int* err) {
-  uint64_t t0 = 0;
-  for (uint32_t i = 1; !mbar_try_wait_sleep(bar, phase & 1); ++i) {
-    if (i & 15) continue;
-    const uint64_t now = globaltimer_ns();
-    if (t0 == 0) t0 = now;
-    if (now - t0 > kWaitLimitNs) {
-      set_dev_error(err, SK_DEVERR_TIMEOUT);
-      return false;
-    }
-  }
-  return true;
-}
-
 // Where the row, head and request coordinates of a cache go in its tensor map, whose dimensions are sorted by
 // stride.
 struct MapOrder {

@@ -39,7 +39,7 @@ def rope_table(n, hd):
 class Step:
     """The tensors of one call, on the GPU."""
 
-    def __init__(self, dev, lens, P, nq, nkv, hd, cdt=BF, io=F32, mass=False, gone=0, slack=9, seed=0, strided=False):
+    def __init__(self, dev, lens, P, nq, nkv, hd, cdt=BF, io=F32, mass=False, gone=0, slack=9, seed=0, strided=0):
         g = torch.Generator().manual_seed(seed)
         R, M = len(lens), max(max(lens) + 1, 1) + slack
         self.nq, self.nkv, self.hd, self.P, self.io, self.lens, self.R, self.M = nq, nkv, hd, P, io, lens, R, M
@@ -49,8 +49,8 @@ class Step:
             for i in range(n):
                 x[i, :, max(used[i], 0):] = math.nan
             x = x.to(cdt)
-            if strided:  # rows of all heads side by side, a gap after each head's part
-                y = torch.full((n, rows, nkv, hd + 16), math.nan, dtype=cdt).to(dev)[..., :hd].permute(0, 2, 1, 3)
+            if strided:  # rows of all heads side by side, a gap of `strided` elements after each head's part
+                y = torch.full((n, rows, nkv, hd + strided), math.nan, dtype=cdt).to(dev)[..., :hd].permute(0, 2, 1, 3)
                 y.copy_(x)
                 return y
             return x.to(dev)
@@ -173,8 +173,9 @@ CASES = {
     "many short requests": dict(lens=[(7 * i) % 50 for i in range(400)], P=40, nq=2, nkv=1, hd=64),
     "the most requests": dict(lens=[(3 * i) % 5 for i in range(1024)], P=5, nq=2, nkv=1, hd=64),
     "evicted before": dict(lens=[500, 131], P=96, nq=16, nkv=8, hd=128, gone=4000),
-    "strided caches": dict(lens=[500, 131, 0], P=96, nq=6, nkv=3, hd=128, strided=True),
-    "strided caches of 64": dict(lens=[500, 131, 0], P=96, nq=6, nkv=3, hd=64, strided=True),
+    "strided caches": dict(lens=[500, 131, 0], P=96, nq=6, nkv=3, hd=128, strided=16),
+    "rows on 16 bytes only": dict(lens=[500, 131, 0], P=96, nq=6, nkv=3, hd=128, strided=8),
+    "strided caches of 64": dict(lens=[500, 131, 0], P=96, nq=6, nkv=3, hd=64, strided=24),
 }
 TYPES = {"bf16 cache, f32 io": (BF, F32), "bf16 cache, bf16 io": (BF, BF), "f32 cache": (F32, F32)}
 
