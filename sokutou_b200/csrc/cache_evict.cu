@@ -1,9 +1,8 @@
 // Key/value caches brought down to a budget of rows by accumulated attention weight.
 //
-// Two kernels. `select`: one CTA per cache (layer, request, head) finds the smallest mass that still fits
-// the budget by radix selection — 11, 11 and 10 bits of the order-preserving integer image of the float
-// from the top, a histogram each, so three reads of the masses whatever the budget — and lists the kept
-// rows in order, one pass that counts and one that writes. `move`: gathers the listed rows of K, V and mass.
+// Two kernels. `select`: one CTA per cache (layer, request, head) finds the smallest mass that still fits the
+// budget by a search over the order-preserving integer image of the float, the keys held in registers, and
+// lists the kept rows in order. `move`: gathers the listed rows of K, V and mass.
 //
 // In place a kept row never moves up (its new index is at most its old one), so a CTA that owns a column
 // slice of a cache can walk the list from the front in batches: a batch's rows are all in registers before
@@ -43,104 +42,157 @@ __device__ __forceinline__ uint32_t key_of(float x) {
   return (b >> 31) ? ~b : (b | 0x80000000u);
 }
 
-constexpr int kSelThreads = 512, kSelWarps = kSelThreads / 32, kBins = 2048;
+// One CTA per cache. Every thread holds eight rows' keys (rows 256 w + 32 i + lane of warp w), loaded before the
+// number of rows is known; caches past 8 * THREADS rows are read again for each block of that many. (Keys in
+// shared memory and short loops over them took a tenth longer.)
+//
+// The threshold is found digit by digit, 8 bits each from the top, a histogram of 256 bins per digit, and the
+// search ends with the first digit whose bin holds as many keys as are still to be kept. The keys are first
+// moved down by the smallest and up to the top bit, which spreads them over the bins of the first digit: two
+// digits are the rule for masses that differ, four the most. (Histograms of 11, 11 and 10 bits of the keys as
+// they are, most of them in a few bins, took a cache of 1536 rows twice as long, and so did a search two bits at
+// a time by warp-wide counts: 800 cycles a step.)
+constexpr int kHeld = 8;  // keys per thread and block
 
-__global__ void __launch_bounds__(kSelThreads) select_kernel(const Params p) {
-  __shared__ int hist[kBins];
-  __shared__ int warp_tot[kSelWarps][2];
-  __shared__ int found_bin, found_above;
-  const int t = threadIdx.x, lane = t & 31, w = t >> 5;
-  const int head = blockIdx.x, kvh = head % p.nkv, r = (head / p.nkv) % p.R, layer = head / (p.nkv * p.R);
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) select_kernel(const Params p) {
+  constexpr int WARPS = THREADS / 32, BLOCK = THREADS * kHeld;
+  __shared__ int hist[2][256];
+  __shared__ uint32_t ends[2][WARPS];
+  __shared__ int tot[8], found[3];
+  __shared__ int2 counts[WARPS];
+  const int t = threadIdx.x, lane = t & 31, w = t >> 5, head = blockIdx.x;
+  const int kvh = head % p.nkv, r = (head / p.nkv) % p.R, layer = head / (p.nkv * p.R);
+  if (t < 256) hist[0][t] = 0;
   griddep_wait();
   griddep_launch_dependents();
+  const float* mass = p.mass + layer * p.ms[0] + r * p.ms[1] + kvh * p.ms[2];
+  const int j0 = w * 32 * kHeld + lane;  // row of this thread's first key in a block
+  uint32_t key[kHeld];
+  auto load = [&](int block, int n) __attribute__((always_inline)) {
+    float x[kHeld];
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const int j = block * BLOCK + j0 + 32 * i;
+      x[i] = j < n ? mass[j] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) key[i] = key_of(x[i]);
+  };
   const long long n64 = p.rows[r];
+  load(0, p.max_len);
   const int n = n64 < 0 || n64 > p.max_len ? -1 : (int)n64;
   if (t == 0 && kvh == 0 && layer == 0) {
     p.cnt[r] = n;
     if (n64 > p.max_len) set_dev_error(p.err, SK_DEVERR_POS_RANGE);
   }
   if (n <= p.keep) return;
-  const float* mass = p.mass + layer * p.ms[0] + r * p.ms[1] + kvh * p.ms[2];
-  const int a = p.first, z = n - p.recent;      // candidates [a, z)
-  int need = p.keep - p.first - p.recent;       // of which this many stay (fewer than there are)
+  const int a = p.first, z = n - p.recent;       // candidates [a, z); the rest of [0, n) stays
+  int need = p.keep - p.first - p.recent;        // of the candidates (fewer than there are)
+  const int blocks = (n + BLOCK - 1) / BLOCK;
+  auto candidate = [&](int block, int i) {
+    const int j = block * BLOCK + j0 + 32 * i;
+    return j >= a && j < z;
+  };
 
-  uint32_t prefix = 0, known = 0;  // the threshold key's leading bits so far and which they are
-  if (need > 0) {
-    const int shifts[3] = {21, 10, 0}, widths[3] = {11, 11, 10};
+  // smallest and largest candidate
+  uint32_t low = 0xffffffffu, high = 0;
+  for (int block = 0; block < blocks; ++block) {
+    if (blocks > 1) load(block, n);
 #pragma unroll
-    for (int pass = 0; pass < 3; ++pass) {
-      for (int i = t; i < kBins; i += kSelThreads) hist[i] = 0;
-      __syncthreads();
-      for (int j = a + t; j < z; j += kSelThreads) {
-        const uint32_t k = key_of(mass[j]);
-        if ((k & known) == prefix) atomicAdd(&hist[(k >> shifts[pass]) & ((1u << widths[pass]) - 1)], 1);
+    for (int i = 0; i < kHeld; ++i)
+      if (candidate(block, i)) {
+        low = min(low, key[i]);
+        high = max(high, key[i]);
       }
-      __syncthreads();
-      // the bin, from the top, in which the count reaches `need`: thread t sums bins 4t .. 4t+3 reversed
-      constexpr int B = kBins / kSelThreads;
-      int own[B], sum = 0;
+  }
+  low = __reduce_min_sync(0xffffffffu, low);
+  high = __reduce_max_sync(0xffffffffu, high);
+  if (lane == 0) ends[0][w] = low, ends[1][w] = high;
+  __syncthreads();
+  low = __reduce_min_sync(0xffffffffu, lane < WARPS ? ends[0][lane] : 0xffffffffu);
+  high = __reduce_max_sync(0xffffffffu, lane < WARPS ? ends[1][lane] : 0u);
+  const int up = __clz((high - low) | 1u);
+  auto moved = [&](uint32_t k) { return (k - low) << up; };  // of a candidate: keeps their order
+
+  uint32_t T = 0;          // leading digits of the threshold
+  bool exact = need == 0;  // exactly as many candidates as are kept reach T
+#pragma unroll 1
+  for (int digit = 0; digit < 4 && !exact; ++digit) {
+    const int shift = 24 - 8 * digit;
+    int* hs = hist[digit & 1];
+    for (int block = 0; block < blocks; ++block) {
+      if (blocks > 1) load(block, n);
 #pragma unroll
-      for (int b = 0; b < B; ++b) {
-        own[b] = hist[kBins - 1 - (t * B + b)];
-        sum += own[b];
+      for (int i = 0; i < kHeld; ++i) {
+        const uint32_t k = moved(key[i]);
+        if (candidate(block, i) && (digit == 0 || (k ^ T) >> (shift + 8) == 0)) atomicAdd(&hs[(k >> shift) & 255], 1);
       }
-      int x = sum;
+    }
+    __syncthreads();
+    int own = 0, x = 0;
+    if (t < 256) {  // bins from the top: how many keys lie in them and above
+      own = x = hs[255 - t];
+      hist[(digit + 1) & 1][t] = 0;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
       }
-      if (lane == 31) warp_tot[w][0] = x;
-      __syncthreads();
-      int above = x - sum;
-      for (int i = 0; i < w; ++i) above += warp_tot[i][0];
-#pragma unroll
-      for (int b = 0; b < B; ++b) {
-        if (above < need && above + own[b] >= need) {
-          found_bin = kBins - 1 - (t * B + b);
-          found_above = above;
-        }
-        above += own[b];
-      }
-      __syncthreads();
-      need -= found_above;
-      prefix |= (uint32_t)found_bin << shifts[pass];
-      known |= ((1u << widths[pass]) - 1) << shifts[pass];
-    }
-  }
-  // kept: first, recent, keys above the threshold `prefix`, and the first `need` of those equal to it.
-  // Each warp takes a run of rows: count, add up the warps before, write.
-  const bool none = p.keep == p.first + p.recent;
-  const int run = ((n + kSelWarps - 1) / kSelWarps + 31) & ~31, j0 = w * run, j1 = min(n, j0 + run);
-  int* list = p.list + (long long)head * p.keep;
-  int sure = 0, ties = 0;
-#pragma unroll 1
-  for (int write = 0; write < 2; ++write) {
-    for (int j = j0; j < j1; j += 32) {
-      const int i = j + lane;
-      const bool end = i < j1 && (i < a || i >= z);
-      const uint32_t k = i < j1 && !end && !none ? key_of(mass[i]) : 0u;
-      const bool mid = i < j1 && !end && !none;
-      const bool s = end || (mid && k > prefix), e = mid && k == prefix;
-      const uint32_t bs = __ballot_sync(0xffffffffu, s), be = __ballot_sync(0xffffffffu, e);
-      if (write) {
-        const uint32_t below = (1u << lane) - 1;
-        const int eb = ties + __popc(be & below);
-        if (s || (e && eb < need)) list[sure + __popc(bs & below) + min(eb, need)] = i;
-      }
-      sure += __popc(bs);
-      ties += __popc(be);
-    }
-    if (write) break;
-    if (lane == 0) {
-      warp_tot[w][0] = sure;
-      warp_tot[w][1] = ties;
+      if (lane == 31) tot[w] = x;
     }
     __syncthreads();
-    sure = ties = 0;
-    for (int i = 0; i < w; ++i) {
-      sure += warp_tot[i][0];
-      ties += warp_tot[i][1];
+    if (t < 256) {
+      x += __reduce_add_sync(0xffffffffu, lane < w ? tot[lane & 7] : 0);
+      if (x >= need && x - own < need) {
+        found[0] = 255 - t;
+        found[1] = x - own;
+        found[2] = own;
+      }
+    }
+    __syncthreads();
+    T |= (uint32_t)found[0] << shift;
+    need -= found[1];
+    exact = need == found[2];
+  }
+  // Kept: the ends, candidates above T (reaching it, if exactly those), and the first `room` that equal it.
+  const int room = exact ? 0 : need;
+  const bool none = p.keep == p.first + p.recent;
+  int* list = p.list + (long long)head * p.keep;
+  int sure = 0, ties = 0;  // of the blocks before
+#pragma unroll 1
+  for (int block = 0; block < blocks; ++block) {
+    if (blocks > 1) load(block, n);
+    uint32_t bs[kHeld], be[kHeld];
+    int own_sure = 0, own_ties = 0;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const int j = block * BLOCK + j0 + 32 * i;
+      const bool mid = j >= a && j < z, end = j < n && !mid;
+      const uint32_t k = moved(key[i]);
+      bs[i] = __ballot_sync(0xffffffffu, end || (mid && !none && (exact ? k >= T : k > T)));
+      be[i] = __ballot_sync(0xffffffffu, room > 0 && mid && k == T);
+      own_sure += __popc(bs[i]);
+      own_ties += __popc(be[i]);
+    }
+    if (lane == 0) counts[w] = make_int2(own_sure, own_ties);
+    __syncthreads();
+    const int2 c = lane < WARPS ? counts[lane] : make_int2(0, 0);
+    int s = sure + __reduce_add_sync(0xffffffffu, lane < w ? c.x : 0);
+    int e = ties + __reduce_add_sync(0xffffffffu, lane < w ? c.y : 0);
+    const uint32_t below = (1u << lane) - 1;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const int eb = e + __popc(be[i] & below);
+      if (((bs[i] >> lane) & 1) || (((be[i] >> lane) & 1) && eb < room))
+        list[s + __popc(bs[i] & below) + min(eb, room)] = block * BLOCK + j0 + 32 * i;
+      s += __popc(bs[i]);
+      e += __popc(be[i]);
+    }
+    if (blocks > 1) {
+      sure += __reduce_add_sync(0xffffffffu, c.x);
+      ties += __reduce_add_sync(0xffffffffu, c.y);
+      __syncthreads();
     }
   }
 }
@@ -200,43 +252,47 @@ __global__ void __launch_bounds__(kMoveThreads) move_in_place_kernel(const Param
   }
 }
 
-// Into another buffer: CTA (cache, K or V, chunk of kCopyRows rows), whole rows.
-constexpr int kCopyRows = 128;
+// Into another buffer: CTA (cache, K or V, chunk of kCopyRows rows), whole rows of U 16-byte units. Four units
+// a thread at a time and 40 registers at most, so that six CTAs share an SM: with eight units and 80 registers
+// three did, and the copy ran at 4.1 TB/s.
+constexpr int kCopyRows = 128, kCopyBatch = 4;
 
-__global__ void __launch_bounds__(kMoveThreads) move_copy_kernel(const Params p) {
+template <int U>
+__global__ void __launch_bounds__(kMoveThreads, 6) move_copy_kernel(const Params p) {
+  constexpr int RPP = kMoveThreads / U;  // rows per pass of the CTA
   const int t = threadIdx.x, head = blockIdx.x;
   const int kvh = head % p.nkv, r = (head / p.nkv) % p.R, layer = head / (p.nkv * p.R);
   const int which = blockIdx.y & 1, d0 = (int)(blockIdx.y >> 1) * kCopyRows;
   griddep_wait();
   griddep_launch_dependents();
+  const int* list = p.list + (long long)head * p.keep;
   const int n = p.cnt[r];
   if (t == 0 && blockIdx.y == 0 && kvh == 0 && layer == 0)
     p.rows_out[r] = n > p.keep ? (long long)p.keep : p.rows[r];
   const int m = min(n, p.keep), d1 = min(m, d0 + kCopyRows);
   if (d0 >= m) return;
   const bool all = n <= p.keep;
-  const int* list = p.list + (long long)head * p.keep;
-  const int U = p.row_bytes / 16;
-  const uint8_t* src = (which ? p.V : p.K) + layer * p.kv[0] + r * p.kv[1] + kvh * p.kv[2];
-  uint8_t* dst = (which ? p.Vo : p.Ko) + layer * p.kvo[0] + r * p.kvo[1] + kvh * p.kvo[2];
-  for (int i0 = 0; i0 < (d1 - d0) * U; i0 += kMoveThreads * kBatch) {
-    uint4 v[kBatch];
+  const uint8_t* src = (which ? p.V : p.K) + layer * p.kv[0] + r * p.kv[1] + kvh * p.kv[2] + (t % U) * 16;
+  uint8_t* dst = (which ? p.Vo : p.Ko) + layer * p.kvo[0] + r * p.kvo[1] + kvh * p.kvo[2] + (t % U) * 16;
+#pragma unroll 1
+  for (int d = d0 + t / U; d < d1; d += RPP * kCopyBatch) {
+    uint4 v[kCopyBatch];
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int i = i0 + b * kMoveThreads + t, d = d0 + i / U;
-      if (d < d1) v[b] = __ldcs(reinterpret_cast<const uint4*>(src + (all ? d : list[d]) * p.kv[3] + (i % U) * 16));
+    for (int b = 0; b < kCopyBatch; ++b) {
+      const int x = d + b * RPP;
+      if (x < d1) v[b] = __ldcs(reinterpret_cast<const uint4*>(src + (all ? x : __ldg(list + x)) * p.kv[3]));
     }
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int i = i0 + b * kMoveThreads + t, d = d0 + i / U;
-      if (d < d1) *reinterpret_cast<uint4*>(dst + d * p.kvo[3] + (i % U) * 16) = v[b];
+    for (int b = 0; b < kCopyBatch; ++b) {
+      const int x = d + b * RPP;
+      if (x < d1) __stcs(reinterpret_cast<uint4*>(dst + x * p.kvo[3]), v[b]);
     }
   }
-  if (which == 0)
-    for (int d = d0 + t; d < d1; d += kMoveThreads)
-      p.mo[layer * p.mso[0] + r * p.mso[1] + kvh * p.mso[2] + d] =
-          p.mass[layer * p.ms[0] + r * p.ms[1] + kvh * p.ms[2] + (all ? d : list[d])];
+  if (which == 0 && d0 + t < d1)
+    p.mo[layer * p.mso[0] + r * p.mso[1] + kvh * p.mso[2] + d0 + t] =
+        p.mass[layer * p.ms[0] + r * p.ms[1] + kvh * p.ms[2] + (all ? d0 + t : __ldg(list + d0 + t))];
 }
+static_assert(kCopyRows <= kMoveThreads, "a mass per thread");
 
 static int check_sizes(const SkCacheEvict* d) {
   if (!d) return SK_ERR_INVALID_ARG;
@@ -337,8 +393,11 @@ extern "C" int sk_cache_evict(const SkCacheEvict* d, void* stream) {
   cfg.numAttrs = 1;
   cfg.stream = reinterpret_cast<cudaStream_t>(stream);
   cfg.gridDim = dim3(heads);
-  cfg.blockDim = dim3(kSelThreads);
-  if (cudaLaunchKernelEx(&cfg, select_kernel, p) != cudaSuccess) return SK_ERR_CUDA;
+  const bool small = d->max_len <= 256 * kHeld;  // small CTAs take less time to synchronise
+  cfg.blockDim = dim3(small ? 256u : d->max_len <= 512 * kHeld ? 512u : 1024u);
+  void (*const select)(const Params) = small                        ? select_kernel<256>
+                                       : d->max_len <= 512 * kHeld ? select_kernel<512> : select_kernel<1024>;
+  if (cudaLaunchKernelEx(&cfg, select, p) != cudaSuccess) return SK_ERR_CUDA;
   cfg.blockDim = dim3(kMoveThreads);
   constexpr int kSlice = 64;
   if (in_place) {
@@ -346,5 +405,7 @@ extern "C" int sk_cache_evict(const SkCacheEvict* d, void* stream) {
     return cudaLaunchKernelEx(&cfg, move_in_place_kernel<kSlice>, p) == cudaSuccess ? SK_OK : SK_ERR_CUDA;
   }
   cfg.gridDim = dim3(heads, (unsigned)(2 * ((d->keep + kCopyRows - 1) / kCopyRows)));
-  return cudaLaunchKernelEx(&cfg, move_copy_kernel, p) == cudaSuccess ? SK_OK : SK_ERR_CUDA;
+  void (*const copy)(const Params) = p.row_bytes == 128   ? move_copy_kernel<8>
+                                     : p.row_bytes == 256 ? move_copy_kernel<16> : move_copy_kernel<32>;
+  return cudaLaunchKernelEx(&cfg, copy, p) == cudaSuccess ? SK_OK : SK_ERR_CUDA;
 }

@@ -221,7 +221,8 @@ __global__ void __launch_bounds__(kJoinThreads, 5) join_kernel(const Params p) {
   const int r = blockIdx.x / p.nkv, kvh = blockIdx.x % p.nkv;
   griddep_launch_dependents();
   bool bad = false;
-  const int n = own_rows(p, r, &bad);
+  int pos = 0;
+  const int n = own_rows(p, r, &bad, &pos);
   if (n < 0 || (blockIdx.y > 0 && (int)blockIdx.y * kMassChunk >= n)) {
     griddep_wait();  // every thread, before any exit: the kernel after this one relies on it
     return;
@@ -250,7 +251,6 @@ __global__ void __launch_bounds__(kJoinThreads, 5) join_kernel(const Params p) {
   float acc[E] = {};
   float m_run = -INFINITY, l_run = 0.f;
   if (h < p.g) {
-    const int pos = (int)p.pos[r];
     const long long base = r * p.qkv_stride;
     RawRow<HD> raw[3];
     raw[0].load(p.qkv, base + (long long)(kvh * p.g + h) * HD, p.qkv_bf16);

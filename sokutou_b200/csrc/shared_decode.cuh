@@ -114,7 +114,7 @@ __host__ inline WsLayout ws_layout(int R, int nq, int nkv, int hd, int P, int ma
 }
 
 // Own rows of request r before this step, -1 if the slot is idle (or out of range: *bad).
-__device__ __forceinline__ int own_rows(const Params& p, int r, bool* bad) {
+__device__ __forceinline__ int own_rows(const Params& p, int r, bool* bad, int* at = nullptr) {
   const long long pos = p.pos[r], own = p.rows ? p.rows[r] : pos - p.P;  // both loads at once
   if (pos < 0) return -1;
   const long long n = own;
@@ -122,16 +122,17 @@ __device__ __forceinline__ int own_rows(const Params& p, int r, bool* bad) {
     *bad = true;
     return -1;
   }
+  if (at) *at = (int)pos;
   return (int)n;
 }
 
 // The row of tiles of one step (the host refuses sizes whose costs could pass 2^31). With many tiles a CTA
 // each tile costs 2^shift and the first of an item `first` more: a segment's query rows have to be read,
 // normalised and written as an operand, and its partials drained. On the tensor cores: own tiles 2, 2 more for
-// the first; prefix tiles of more than kFewRows query rows 4, 4 more for the first (they take the tensor cores
-// and the exponentials for about twice as long, and their rows are many; with every tile at 1 the prefix's
-// CTAs took 133 thousand cycles when the others took 75, at 64 requests behind 8192 rows). With fewer tiles
-// each costs 1 and is a CTA's own.
+// the first; prefix tiles of more than kFewRows query rows 4, and 4 more for the first, 8 above 64 rows (they
+// take the tensor cores and the exponentials for about twice as long, and their rows are many). With every
+// tile at 1 the prefix's CTAs took 133 thousand cycles when the others took 75, at 64 requests behind 8192 rows
+// (74 us, 54.7 so; 60.7 with 4 in the place of 8, 59.0 with 12). With fewer tiles each costs 1 and is a CTA's own.
 constexpr int kFewRows = 8;
 
 struct Tiles {
@@ -152,10 +153,10 @@ __device__ __forceinline__ Tiles tiles_of(const Params& p, int own_tiles, int ow
   t.items_p = t.tp > 0 ? t.nrt * p.nkv : 0;
   const bool many = rows > kFewRows;
   t.shift_o = 1, t.first_o = 2;
-  t.shift_p = many ? 2 : 1, t.first_p = many ? 4 : 2;
+  t.shift_p = many ? 2 : 1, t.first_p = many ? (rows > 64 ? 8 : 4) : 2;
   int total = t.items_p * t.cost_p() + p.nkv * (own_items * t.first_o + (own_tiles << t.shift_o));
   // no share may be without a tile's start: a share costs at least what lies between two starts
-  if (!Cut::kWeighted || total < Cut::G * (t.items_p && many ? 8 : 4)) {
+  if (!Cut::kWeighted || total < Cut::G * (t.items_p ? (t.first_p + (1 << t.shift_p)) : 4)) {
     t.shift_o = t.first_o = t.shift_p = t.first_p = 0;
     total = t.items_p * t.tp + p.nkv * own_tiles;
   }
@@ -189,9 +190,10 @@ __device__ __forceinline__ Tiles scan_tiles(const Params& p, const Lens& s, bool
   int tiles = 0, items = 0, live = 0;
 #pragma unroll 4
   for (int r = lane; r < p.R; r += 32) {  // no iteration waits for another's loads
-    const int n = own_rows(p, r, &bad);
+    int at = 0;
+    const int n = own_rows(p, r, &bad, &at);
     s.len[r] = n;
-    s.pos[r] = n >= 0 ? (int)p.pos[r] : 0;
+    s.pos[r] = at;
     tiles += n > 0 ? (n + KT - 1) / KT : 0;
     items += n > 0;
     live += n >= 0;

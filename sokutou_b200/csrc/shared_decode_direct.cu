@@ -5,16 +5,20 @@
 // running maximum is a warp's and moves only when a score exceeds it by 2^8.
 //
 // bf16 caches: every warp copies its own batches of 16 keys (8 KB) to shared memory, two ahead of the one that it
-// works on, with the warp-wide tensor instruction (mma.m16n8k16). Its 16
-// rows are the 8 query heads of a group twice, q as hi + lo bf16 terms (2^-16 of q is left out at most), so a
-// thread gets the two parts of a score in its own registers; the weights take the same places, hi rows and lo
-// rows, as the left operand of the value product. The inner index of a product may run over the elements in
-// any order, so K is read 16 bytes a lane as it lies and q laid out to match. 16 keys (8 KB) take about 130
-// instructions; multiplied element by element they took a thousand, and from registers, without the copies,
-// the loads in flight were too few.
+// works on, with the warp-wide tensor instruction (mma.m16n8k16): its 16 rows are the 8 query heads of a group
+// twice, q's first bf16 terms and its second, so a thread gets the two parts of a score in its own registers, and
+// the weights take the same places as the left operand of the value product. Two terms leave out 2^-16 of a
+// number at most. Where fp32 goes out or weights are kept q has a third term (2^-24), in rows that up to four heads
+// leave free; the weights' rest is rounded off evenly over the keys and stays. The inner index of a product may
+// run over the elements in any order, so K is read 16 bytes a lane as it lies and q laid out to match. 16
+// keys take some 140 instructions; multiplied element by element they took a thousand, and straight from global
+// memory to registers the loads in flight were too few (16 slots behind 96 rows, 1404 rows the longest: 18.7 us so,
+// 18.5 and 23.7 the other ways; one stream of 1119 rows with its weights: 8.6, 9.4 and 9.5 us).
 //
 // fp32 caches: element by element; a row takes 16 or 32 lanes, every lane multiplies its elements for all
 // heads, one butterfly leaves each sum in one lane, which exponentiates it, and shuffles bring the weights back.
+#include <type_traits>
+
 #include "shared_decode.cuh"
 
 namespace sk {
@@ -179,10 +183,15 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-// x's two bf16 terms, a pair at a time
-__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
-  hi = pack2(a, b);
-  lo = pack2(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u));
+// The bf16 terms of a pair, each of what the ones before leave.
+template <int N>
+__device__ __forceinline__ void split(float a, float b, uint32_t (&x)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    x[i] = pack2(a, b);
+    a -= __uint_as_float(x[i] << 16);
+    b -= __uint_as_float(x[i] & 0xffff0000u);
+  }
 }
 __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&d)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -196,25 +205,31 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool k
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(keep ? 16 : 0) : "memory");
 }
 
-template <int HD>
+// How q's third term is taken: not at all (bf16 out and no weights kept, which two terms are exact enough for),
+// in rows of the product that four heads leave free, or in products of its own.
+enum Third { kNoThird, kInRows, kApart };
+
+template <int HD, Third THIRD>
 struct MmaSmem {
   static constexpr int kRows = 16;                // keys of a batch
   // Batches in a warp's ring, CTAs per SM (measured, graph: 16 slots of 128 18.1 us with 3 and 2 against 20.0
   // with 2 and 3; 45 requests of 4 heads of 64 21.9 us with 4 and 3 against 29.1 with 6 and 2).
-  static constexpr int NST = HD == 128 ? 3 : 4, kPerSm = HD == 128 ? 2 : 3;
+  static constexpr int NST = HD == 128 ? 3 : 4, kPerSm = HD == 128 || THIRD == kApart ? 2 : 3;
   static constexpr int PITCH = HD * 2 + 16;       // bytes: an odd number of 16-byte units, no bank conflicts
   static constexpr int HALF = kRows * PITCH, SLOT = 2 * HALF;  // K, V
-  static constexpr int OFF_Q = kMmaWarps * NST * SLOT;           // [hi, lo][8 rows][PITCH]
-  static constexpr int OFF_NEW = OFF_Q + 2 * kMaxGroup * PITCH;  // the new token's k and v
+  static constexpr int kTerms = THIRD == kApart ? 3 : 2;
+  static constexpr int OFF_Q = kMmaWarps * NST * SLOT;                // [kTerms][8 rows][PITCH]: see the kernel
+  static constexpr int OFF_NEW = OFF_Q + kTerms * kMaxGroup * PITCH;  // the new token's k and v
   static constexpr int BYTES = OFF_NEW + 2 * HD * 2;
   // after the last batch the rings hold the warps' outputs and the CTA's
   static constexpr int OFF_RED = 0, OFF_O = kMmaWarps * kMaxGroup * HD * 4;
   static_assert(OFF_O + kMaxGroup * HD * 4 <= OFF_Q, "the outputs fit the rings");
+  static_assert(kPerSm * (BYTES + 512 + 1024) <= 233472, "that many CTAs share an SM's shared memory");
 };
 
-template <int HD>
-__global__ void __launch_bounds__(kMmaThreads, MmaSmem<HD>::kPerSm) direct_mma_kernel(const Params p, int cluster) {
-  using S = MmaSmem<HD>;
+template <int HD, Third THIRD>
+__global__ void __launch_bounds__(kMmaThreads, MmaSmem<HD, THIRD>::kPerSm) direct_mma_kernel(const Params p, int cluster) {
+  using S = MmaSmem<HD, THIRD>;
   constexpr int GP = kMaxGroup, EL = HD / 32, NST = S::NST, kRows = S::kRows;
   constexpr int NP = HD / 32;  // 16-byte pieces of a K row per lane: elements 32 i + 8 (lane % 4) ...
   constexpr int U = HD / 8, RPI = 32 / U;  // 16-byte units of a row, rows per instruction of a warp's copy
@@ -272,11 +287,14 @@ __global__ void __launch_bounds__(kMmaThreads, MmaSmem<HD>::kPerSm) direct_mma_k
   for (int i = 0; i < NST - 1; ++i) fetch(b0 + w + i * kMmaWarps, i);
 
   // q, and the new token's k and v
-  for (int x = w; x < GP; x += kMmaWarps)  // the rows of heads that are not there
-    if (x >= g && lane < U) {
-      *reinterpret_cast<uint4*>(smem + S::OFF_Q + x * S::PITCH + lane * 16) = make_uint4(0, 0, 0, 0);
-      *reinterpret_cast<uint4*>(smem + S::OFF_Q + (GP + x) * S::PITCH + lane * 16) = make_uint4(0, 0, 0, 0);
-    }
+  // The product's rows 0-7 and 8-15 are q_s[0] and q_s[1]: head h's first term in row h, its second in row 8 + h,
+  // its third in row 4 + h (kInRows) or in q_s[2] (kApart); the rows left over are zero.
+  constexpr int kTerms = THIRD == kNoThird ? 2 : 3;
+  for (int x = w; x < S::kTerms * GP; x += kMmaWarps) {
+    const int y = x % GP;
+    const bool used = y < g || (THIRD == kInRows && x < GP && y >= 4 && y < 4 + g);
+    if (!used && lane < U) *reinterpret_cast<uint4*>(smem + S::OFF_Q + x * S::PITCH + lane * 16) = make_uint4(0, 0, 0, 0);
+  }
   for (int x = w; x < g + 2; x += kMmaWarps) {
     if (x != w) raw[0].load(p.qkv, source(x), p.qkv_bf16);
     float y[1][EL];
@@ -289,10 +307,13 @@ __global__ void __launch_bounds__(kMmaThreads, MmaSmem<HD>::kPerSm) direct_mma_k
     if (x < g) {
 #pragma unroll
       for (int e = 0; e < EL; e += 2) {
-        uint32_t hi, lo;
-        split2(y[0][e] * p.q_scale, y[0][e + 1] * p.q_scale, hi, lo);
-        *reinterpret_cast<uint32_t*>(smem + S::OFF_Q + x * S::PITCH + (lane * EL + e) * 2) = hi;
-        *reinterpret_cast<uint32_t*>(smem + S::OFF_Q + (GP + x) * S::PITCH + (lane * EL + e) * 2) = lo;
+        uint32_t term[kTerms];
+        split(y[0][e] * p.q_scale, y[0][e + 1] * p.q_scale, term);
+        uint8_t* dst = smem + S::OFF_Q + (lane * EL + e) * 2;
+        *reinterpret_cast<uint32_t*>(dst + x * S::PITCH) = term[0];
+        *reinterpret_cast<uint32_t*>(dst + (GP + x) * S::PITCH) = term[1];
+        if (THIRD != kNoThird)
+          *reinterpret_cast<uint32_t*>(dst + (THIRD == kApart ? 2 * GP + x : 4 + x) * S::PITCH) = term[kTerms - 1];
       }
     } else {
       __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(x == g ? p.Kc : p.Vc) + own_at + n * p.row_stride + lane * EL;
@@ -306,8 +327,9 @@ __global__ void __launch_bounds__(kMmaThreads, MmaSmem<HD>::kPerSm) direct_mma_k
   }
   __syncthreads();
 
-  float m = -INFINITY, l = 0.f;  // of head `row`, the same in its four lanes / this lane's part
-  float o[HD / 8][4];            // head `row`: elements 8 t + 2c, + 1 by hi weights, then by lo
+  const int h = THIRD == kInRows ? row & 3 : row;  // this lane's head (rows 4-7 keep step with 0-3, to no effect)
+  float m = -INFINITY, l = 0.f;  // of head h, the same in its four lanes / this lane's part
+  float o[HD / 8][4];            // elements 8 t + 2c, + 1 by the weights' first terms, then by their second
 #pragma unroll
   for (int t = 0; t < HD / 8; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
   float* sc = p.mass && row < g ? p.sc + ((long long)r * p.nq + kvh * g + row) * p.sc_stride : nullptr;
@@ -345,6 +367,11 @@ __global__ void __launch_bounds__(kMmaThreads, MmaSmem<HD>::kPerSm) direct_mma_k
         const uint4 k = *reinterpret_cast<const uint4*>(k_at + 8 * u * S::PITCH + 64 * i);
         mma_bf16(s[u], hi.x, lo.x, hi.y, lo.y, k.x, k.y);
         mma_bf16(s2[u], hi.z, lo.z, hi.w, lo.w, k.z, k.w);
+        if (THIRD == kApart) {
+          const uint4 third = *reinterpret_cast<const uint4*>(q_at + 2 * GP * S::PITCH + 64 * i);
+          mma_bf16(s[u], third.x, 0, third.y, 0, k.x, k.y);
+          mma_bf16(s2[u], third.z, 0, third.w, 0, k.z, k.w);
+        }
       }
     }
     bool over = false;
@@ -353,8 +380,10 @@ __global__ void __launch_bounds__(kMmaThreads, MmaSmem<HD>::kPerSm) direct_mma_k
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int j = 8 * u + 2 * c + e;
-        s[u][e] = j < valid ? (s[u][e] + s2[u][e]) + (s[u][2 + e] + s2[u][2 + e]) : -INFINITY;
-        over |= row < g && s[u][e] > m + 8.0f;
+        float x = (s[u][e] + s2[u][e]) + (s[u][2 + e] + s2[u][2 + e]);
+        if (THIRD == kInRows) x += __shfl_xor_sync(0xffffffffu, x, 16);  // rows h and 4 + h
+        s[u][e] = j < valid ? x : -INFINITY;
+        over |= h < g && s[u][e] > m + 8.0f;
         if (sc && own && j < valid) sc[j0 + j] = s[u][e];
       }
     if (__any_sync(0xffffffffu, over)) {
@@ -370,12 +399,15 @@ __global__ void __launch_bounds__(kMmaThreads, MmaSmem<HD>::kPerSm) direct_mma_k
         for (int e = 0; e < 4; ++e) o[x][e] *= a;
     }
     const float use = m == -INFINITY ? 0.f : m;
-    uint32_t a[4];  // left operand: hi rows (keys of u = 0), lo rows, hi rows (u = 1), lo rows
+    uint32_t a[4];  // left operand: rows 0-7 (first terms) for the keys of u = 0, rows 8-15 (second), the same for u = 1
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const float x = ex2_approx(s[u][0] - use), y = ex2_approx(s[u][1] - use);
       l += x + y;
-      split2(x, y, a[2 * u], a[2 * u + 1]);
+      uint32_t term[2];
+      split(x, y, term);
+      a[2 * u] = term[0];
+      a[2 * u + 1] = term[1];
     }
 #pragma unroll
     for (int t = 0; t < HD / 8; t += 2) {
@@ -389,7 +421,7 @@ __global__ void __launch_bounds__(kMmaThreads, MmaSmem<HD>::kPerSm) direct_mma_k
 
   l += __shfl_xor_sync(0xffffffffu, l, 1);
   l += __shfl_xor_sync(0xffffffffu, l, 2);
-  if (c == 0) ml_s[w][row] = make_float2(m, l);
+  if (c == 0) ml_s[w][row] = make_float2(m, l);  // (rows past g are not read)
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();  // every batch read: the rings take the outputs
   if (row < g) {
@@ -675,14 +707,24 @@ int launch_direct(const Params& p, int hd, cudaStream_t st) {
   // length, so that long requests get more CTAs than short ones, took longer: 19 to 29 us for 16 slots of 1 to
   // 1404 rows against 18, clusters of which most CTAs leave at once being slow to start.)
   const int per = p.f32 ? (hd == 128 ? 4 : 8) : 16, warps = p.f32 ? kDirWarps : kMmaWarps;
-  const int slots = 148 * (p.f32 ? 2 : hd == 128 ? MmaSmem<128>::kPerSm : MmaSmem<64>::kPerSm);
+  const Third third = p.out_bf16 && !p.mass ? kNoThird : p.g <= 4 ? kInRows : kApart;
+  const int slots = 148 * (p.f32 || hd == 128 || third == kApart ? 2 : MmaSmem<64, kInRows>::kPerSm);
   const long long heads = (long long)p.R * p.nkv, most = (p.P + per - 1) / per + p.max_len / per + 1;  // batches
   int cluster = 1;
   while (cluster < kMaxCluster && heads * cluster * 2 <= slots && most > cluster * warps) cluster *= 2;
   if (p.f32)
     return launch(hd == 128 ? f32_kernel<128>(p.g) : f32_kernel<64>(p.g), kDirThreads, 0, p, cluster, st);
-  return hd == 128 ? launch(direct_mma_kernel<128>, kMmaThreads, MmaSmem<128>::BYTES, p, cluster, st)
-                   : launch(direct_mma_kernel<64>, kMmaThreads, MmaSmem<64>::BYTES, p, cluster, st);
+  const auto run = [&](auto wide, auto how) {
+    constexpr int HD = decltype(wide)::value;
+    constexpr Third THIRD = decltype(how)::value;
+    return launch(direct_mma_kernel<HD, THIRD>, kMmaThreads, MmaSmem<HD, THIRD>::BYTES, p, cluster, st);
+  };
+  const auto pick = [&](auto wide) {
+    return third == kNoThird  ? run(wide, std::integral_constant<Third, kNoThird>())
+           : third == kInRows ? run(wide, std::integral_constant<Third, kInRows>())
+                              : run(wide, std::integral_constant<Third, kApart>());
+  };
+  return hd == 128 ? pick(std::integral_constant<int, 128>()) : pick(std::integral_constant<int, 64>());
 }
 
 }  // namespace shared

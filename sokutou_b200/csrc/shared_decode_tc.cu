@@ -69,9 +69,10 @@ struct SmemTc {
   static constexpr int OFF_K = OFF_V + NSV * KV_BYTES;
   static constexpr int OFF_ML = OFF_K + NSK * KV_BYTES;  // [2] n > 8: [128] (max, sum of A), [128] sum of B;
   static constexpr int ML_FLOATS = 3 * 128;              //     n <= 8: sums [4][8], max [8]
-  static constexpr int OFF_MX = OFF_ML + 2 * ML_FLOATS * 4;  // n > 8: [2][2][128] maxima of A's and B's halves;
-                                                         // n <= 8: [4][8] of the warps, [8] running, [8] factors
-  static constexpr int OFF_BAR = OFF_MX + 4 * 128 * 4;
+  // n > 8: [2][2][128] maxima of A's and B's halves. n <= 8, in a place of its own, as the warps pass from one
+  // form to the other each in its time: [4][8] maxima of the warps, [8] running, [8] factors.
+  static constexpr int OFF_MX = OFF_ML + 2 * ML_FLOATS * 4, OFF_MK = OFF_MX + 4 * 128 * 4;
+  static constexpr int OFF_BAR = OFF_MK + 48 * 4;
   static constexpr int NBAR = 2 * NSK + 2 * NSV + 16;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;    // tensor-memory base, whether there is a segment
   static constexpr int OFF_TILES = OFF_MISC + 16;
@@ -490,7 +491,7 @@ __global__ void __maxnreg__(kLaunchRegs)
       // n <= 8 query rows, H >= n of them computed
       auto by_keys = [&](auto rows, int n) {
         constexpr int H = decltype(rows)::value;
-        float *m_s = mx_s + 32, *a_s = mx_s + 40;
+        float *mk_s = reinterpret_cast<float*>(smem + S::OFF_MK), *m_s = mk_s + 32, *a_s = mk_s + 40;
         float l[H] = {};
         float* sc = !sg.prefix && p.mass ? p.sc + ((long long)sg.r * p.nq + sg.kvh * p.g) * p.sc_stride + j : nullptr;
         for (int t = sg.t0; t < sg.t1; ++t, ++i) {
@@ -520,11 +521,11 @@ __global__ void __maxnreg__(kLaunchRegs)
 #pragma unroll
             for (int h = 0; h < H; ++h) y[h] = x[h];
             const float top = warp_reduce<H>(y, [](float a, float b) { return fmaxf(a, b); });
-            if (lane % (32 / H) == 0) mx_s[warp * 8 + lane / (32 / H)] = top;
+            if (lane % (32 / H) == 0) mk_s[warp * 8 + lane / (32 / H)] = top;
             named_bar_sync(2, 128);
             if (j < H) {
               const float old = t > sg.t0 ? m_s[j] : -INFINITY;
-              const float to = fmaxf(fmaxf(fmaxf(mx_s[j], mx_s[8 + j]), fmaxf(mx_s[16 + j], mx_s[24 + j])), old);
+              const float to = fmaxf(fmaxf(fmaxf(mk_s[j], mk_s[8 + j]), fmaxf(mk_s[16 + j], mk_s[24 + j])), old);
               a_s[j] = to == -INFINITY ? 1.f : ex2_approx(old - to);
               m_s[j] = to;
             }
@@ -617,7 +618,8 @@ __global__ void __maxnreg__(kLaunchRegs)
           named_bar_sync(3, 256);  // both halves read, so P may go over them, and both maxima written
           if (any) {
             const float m_new = max3(m_run, mine, mx_s[w * 256 + (1 - is_b) * 128 + j]);
-            if (__any_sync(0xffffffffu, m_new > m_run + kRescale)) {  // O and the sum of this warp's rows
+            // (rows that are not the segment's hold anything: they have no say in when)
+            if (__any_sync(0xffffffffu, j >= base && j < base + n && m_new > m_run + kRescale)) {  // O and the sums
               const float alpha = m_new == -INFINITY ? 1.f : ex2_approx(m_run - m_new);
               if (t > sg.t0) {
                 wait(&o_done[(i - 1) & 1], (i - 1) >> 1);
