@@ -8,10 +8,9 @@
 // works on, with the warp-wide tensor instruction (mma.m16n8k16): its 16 rows are the 8 query heads of a group
 // twice, q's first bf16 terms and its second, so a thread gets the two parts of a score in its own registers, and
 // the weights take the same places as the left operand of the value product. Two terms leave out 2^-16 of a
-// number at most. Where fp32 goes out or weights are kept q has a third term (2^-24), in rows that up to four heads
-// leave free; the weights' rest is rounded off evenly over the keys and stays. The inner index of a product may
-// run over the elements in any order, so K is read 16 bytes a lane as it lies and q laid out to match. 16
-// keys take some 140 instructions; multiplied element by element they took a thousand, and straight from global
+// number at most; where fp32 goes out or weights are kept both have a third (2^-24), in rows that up to four heads
+// leave free. The inner index of a product may run over the elements in any order, so K is read 16 bytes a lane
+// as it lies and q laid out to match. 16 keys take some 150 instructions; multiplied element by element they took a thousand, and straight from global
 // memory to registers the loads in flight were too few (16 slots behind 96 rows, 1404 rows the longest: 18.7 us so,
 // 18.5 and 23.7 the other ways; one stream of 1119 rows with its weights: 8.6, 9.4 and 9.5 us).
 //
@@ -327,9 +326,9 @@ __global__ void __launch_bounds__(kMmaThreads, MmaSmem<HD, THIRD>::kPerSm) direc
   }
   __syncthreads();
 
-  const int h = THIRD == kInRows ? row & 3 : row;  // this lane's head (rows 4-7 keep step with 0-3, to no effect)
+  const int h = THIRD == kInRows ? row & 3 : row;  // this lane's head (rows 4-7 keep step with 0-3)
   float m = -INFINITY, l = 0.f;  // of head h, the same in its four lanes / this lane's part
-  float o[HD / 8][4];            // elements 8 t + 2c, + 1 by the weights' first terms, then by their second
+  float o[HD / 8][4];            // elements 8 t + 2c, + 1 by the weights' first (or third) terms, then by their second
 #pragma unroll
   for (int t = 0; t < HD / 8; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
   float* sc = p.mass && row < g ? p.sc + ((long long)r * p.nq + kvh * g + row) * p.sc_stride : nullptr;
@@ -399,15 +398,18 @@ __global__ void __launch_bounds__(kMmaThreads, MmaSmem<HD, THIRD>::kPerSm) direc
         for (int e = 0; e < 4; ++e) o[x][e] *= a;
     }
     const float use = m == -INFINITY ? 0.f : m;
-    uint32_t a[4];  // left operand: rows 0-7 (first terms) for the keys of u = 0, rows 8-15 (second), the same for u = 1
+    // left operand: rows 0-7 for the keys of u = 0, rows 8-15, the same for u = 1; third terms where q's are
+    uint32_t a[4], a3[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const float x = ex2_approx(s[u][0] - use), y = ex2_approx(s[u][1] - use);
       l += x + y;
-      uint32_t term[2];
+      uint32_t term[kTerms];
       split(x, y, term);
-      a[2 * u] = term[0];
-      a[2 * u + 1] = term[1];
+      const bool third = THIRD == kInRows && row >= 4;
+      a[2 * u] = third ? term[kTerms - 1] : term[0];
+      a[2 * u + 1] = third ? 0u : term[1];
+      a3[u] = term[kTerms - 1];
     }
 #pragma unroll
     for (int t = 0; t < HD / 8; t += 2) {
@@ -415,6 +417,10 @@ __global__ void __launch_bounds__(kMmaThreads, MmaSmem<HD, THIRD>::kPerSm) direc
       ldmatrix_x4_trans(vb, ring + slot * S::SLOT + v_at + t * 16);
       mma_bf16(o[t], a[0], a[1], a[2], a[3], vb[0], vb[1]);
       mma_bf16(o[t + 1], a[0], a[1], a[2], a[3], vb[2], vb[3]);
+      if (THIRD == kApart) {
+        mma_bf16(o[t], a3[0], 0, a3[1], 0, vb[0], vb[1]);
+        mma_bf16(o[t + 1], a3[0], 0, a3[1], 0, vb[2], vb[3]);
+      }
     }
     slot = slot == NST - 1 ? 0 : slot + 1;
   }
@@ -424,11 +430,15 @@ __global__ void __launch_bounds__(kMmaThreads, MmaSmem<HD, THIRD>::kPerSm) direc
   if (c == 0) ml_s[w][row] = make_float2(m, l);  // (rows past g are not read)
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();  // every batch read: the rings take the outputs
-  if (row < g) {
 #pragma unroll
-    for (int t = 0; t < HD / 8; ++t)
-      *reinterpret_cast<float2*>(smem + S::OFF_RED + (((w * GP + row) * HD) + 8 * t + 2 * c) * 4) =
-          make_float2(o[t][0] + o[t][2], o[t][1] + o[t][3]);
+  for (int t = 0; t < HD / 8; ++t) {
+    float x = o[t][0] + o[t][2], y = o[t][1] + o[t][3];
+    if (THIRD == kInRows) {  // row 4 + h
+      x += __shfl_xor_sync(0xffffffffu, x, 16);
+      y += __shfl_xor_sync(0xffffffffu, y, 16);
+    }
+    if (row < g)
+      *reinterpret_cast<float2*>(smem + S::OFF_RED + (((w * GP + row) * HD) + 8 * t + 2 * c) * 4) = make_float2(x, y);
   }
   finish<GP, HD, kMmaWarps, kMmaThreads>(p, cluster > 1, active, rank, r, kvh, n, max(0, b0 - nbp) * kRows, min(n + 1, (b1 - nbp) * kRows),
                                          &ml_s[0][0], reinterpret_cast<const float*>(smem + S::OFF_RED),

@@ -11,8 +11,8 @@
 //   warp 15           the scan of the lengths at the start.
 //
 // Two forms of the products, by the segment's query rows n:
-//   n <= 8  S^T = K·Q^T and O^T = V^T·P^T: M = 128 are the tile's keys (the head's elements), N = 16 the query
-//           rows' hi and lo terms side by side. Thread j of softmax A owns key j of the tile; P^T goes to shared
+//   n <= 8  S^T = K·Q^T and O^T = V^T·P^T: M = 128 are the tile's keys (the head's elements), N = 16 or 32 the
+//           query rows' terms side by side. Thread j of softmax A owns key j of the tile; P^T goes to shared
 //           memory; the running maximum is shared by the 128 threads and moved only when a score exceeds it by
 //           2^8, so a tile costs one vote. All own rows (g <= 8 query heads per key) run here: of a 128-row
 //           operand 2 rows would use 1/64.
@@ -20,10 +20,12 @@
 //           keys of a tile, B the others; they exchange their maxima; P stays in tensor memory, over the
 //           scores it came from.
 //
-// Rounding. K and V are bf16 already. q = hi + lo in bf16 leaves 2^-16 of q at most, and costs one more
-// product per tile, which runs while memory is waited for; with a single bf16 term a score of 10 is off by
-// 0.02. The weights P are rounded to bf16 where the output is (2^-8 either way); P_SPLIT (fp32 outputs) adds
-// their rest as a second bf16 term. The running sum is of the unrounded weights, in fp32.
+// Rounding. K and V are bf16 already. q as two bf16 terms leaves 2^-16 of it at most, and the second costs one
+// more product per tile, which runs while memory is waited for; with a single term a score of 10 is off by 0.02.
+// The weights P are rounded to bf16 where the output is (2^-8 either way); P_SPLIT (fp32 outputs) takes them in two
+// terms as well, and with n <= 8, where they are columns that are there anyway, q and P in three (2^-24, as fp32).
+// With n > 8 neither shared nor tensor memory has room for a third: 4e-6 of the output, measured, against 5e-7.
+// The running sum is of the unrounded weights, in fp32.
 #include <type_traits>
 
 #include "shared_decode.cuh"
@@ -60,12 +62,15 @@ struct SmemTc {
   static constexpr int NSK = HD == 128 ? 2 : 4, NSV = HD == 128 ? 2 : 4;
   static constexpr int NCH = HD / 64;
   static constexpr int Q_BYTES = 128 * HD * 2, KV_BYTES = 128 * HD * 2;
-  static constexpr int OFF_Q = 0;  // n > 8: hi rows, then lo rows [128][hd], 64-element chunks 16 KB apart
-  // n <= 8: two buffers of 16 rows (8 hi, 8 lo), two of P^T [16 rows][128 keys], 64-element chunks 2 KB apart
-  static constexpr int QT_BYTES = 16 * HD * 2, PT_BYTES = 16 * 128 * 2;
-  static constexpr int OFF_QT = OFF_Q + 2 * Q_BYTES, OFF_PT = OFF_QT + 2 * QT_BYTES;
+  // Query area. n > 8: hi rows, then lo rows [128][hd], 64-element chunks 16 KB apart. n <= 8: two buffers of 24
+  // rows (8 of each term) and two of P^T [24 rows][128 keys], 64-element chunks 3 KB apart; a product reads 32
+  // rows, the last 8 whatever comes next, for columns that are not used.
+  static constexpr int OFF_Q = 0, CHUNK = 24 * 128;
+  static constexpr int QT_BYTES = NCH * CHUNK, PT_BYTES = 2 * CHUNK;
+  static constexpr int OFF_QT = OFF_Q, OFF_PT = OFF_QT + 2 * QT_BYTES;
+  static_assert(OFF_PT + 2 * PT_BYTES + 1024 <= 2 * Q_BYTES, "the query area holds either form");
   // V before K: at hd = 64 the V^T operand (M = 128) reads 16 KB past its tile, into lanes that are not used
-  static constexpr int OFF_V = OFF_PT + 2 * PT_BYTES;
+  static constexpr int OFF_V = OFF_Q + 2 * Q_BYTES;
   static constexpr int OFF_K = OFF_V + NSV * KV_BYTES;
   static constexpr int OFF_ML = OFF_K + NSK * KV_BYTES;  // [2] n > 8: [128] (max, sum of A), [128] sum of B;
   static constexpr int ML_FLOATS = 3 * 128;              //     n <= 8: sums [4][8], max [8]
@@ -80,7 +85,7 @@ struct SmemTc {
   static constexpr int OFF_LENS = OFF_SEG + 48;
   static_assert(sizeof(Tiles) <= 48 && sizeof(Segments) <= 48, "their places in shared memory");
   static __host__ __device__ int bytes(int R) { return OFF_LENS + Lens::bytes(R); }
-  static_assert(OFF_QT % 1024 == 0 && OFF_PT % 1024 == 0 && OFF_V % 1024 == 0, "swizzled tiles lie on 1024 bytes");
+  static_assert(CHUNK % 1024 == 0 && OFF_V % 1024 == 0, "swizzled tiles lie on 1024 bytes");
   static_assert(OFF_LENS + (3 * kMaxRequests + 1) * 4 <= 232448, "shared memory over the 227 KB per-CTA limit");
 };
 
@@ -184,6 +189,7 @@ __global__ void __maxnreg__(kLaunchRegs)
                     const __grid_constant__ TcArgs args) {
   using S = SmemTc<HD>;
   constexpr int NSK = S::NSK, NSV = S::NSV, NCH = S::NCH, E = HD / 32;
+  constexpr int kCols = P_SPLIT ? 32 : 16;  // columns of the products of few rows: 8 per term, 8 more to the next 16
   const Params& p = args.p;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sbase = smem_u32(smem);
@@ -278,25 +284,30 @@ __global__ void __maxnreg__(kLaunchRegs)
       for (int b = 0; b < kRowsAhead; ++b) {
         const int i = i0 + step * b;
         if (i >= n) break;
-        uint32_t hi[E / 2], lo[E / 2];
+        uint32_t term[3][E / 2];
 #pragma unroll
         for (int e = 0; e < E / 2; ++e) {
-          const float u = x[b][2 * e] * p.q_scale, v = x[b][2 * e + 1] * p.q_scale;
-          hi[e] = pack_bf16(u, v);
-          lo[e] = pack_bf16(lo_part(u, hi[e], 0), lo_part(v, hi[e], 1));
+          float u = x[b][2 * e] * p.q_scale, v = x[b][2 * e + 1] * p.q_scale;
+#pragma unroll
+          for (int i = 0; i < 3; ++i) {
+            term[i][e] = pack_bf16(u, v);
+            u = lo_part(u, term[i][e], 0);
+            v = lo_part(v, term[i][e], 1);
+          }
         }
         // element d: 64-element chunk d / 64, 16-byte unit (d % 64) / 8 exclusive-or the row's low bits
         const int d = lane * E, unit = (d & 63) >> 3, chunk = d >> 6;
         const int in_row = (base + i) * 128 + ((unit ^ (i & 7)) << 4) + (d & 7) * 2;
-        const int at_hi = few ? S::OFF_QT + (seg & 1) * S::QT_BYTES + chunk * 2048 + in_row : S::OFF_Q + chunk * 16384 + in_row;
-        const int at_lo = at_hi + (few ? kFew * 128 : S::Q_BYTES);
-        if (SK_INB(at_lo + 2 * E <= S::OFF_PT, p.err)) {
-          if constexpr (E == 4) {
-            *reinterpret_cast<uint2*>(smem + at_hi) = make_uint2(hi[0], hi[1]);
-            *reinterpret_cast<uint2*>(smem + at_lo) = make_uint2(lo[0], lo[1]);
-          } else {
-            *reinterpret_cast<uint32_t*>(smem + at_hi) = hi[0];
-            *reinterpret_cast<uint32_t*>(smem + at_lo) = lo[0];
+        const int at = few ? S::OFF_QT + (seg & 1) * S::QT_BYTES + chunk * S::CHUNK + in_row : S::OFF_Q + chunk * 16384 + in_row;
+        const int next = few ? kFew * 128 : S::Q_BYTES;  // from one term to the next
+        if (SK_INB(at + next + 2 * E <= 2 * S::Q_BYTES, p.err)) {
+#pragma unroll
+          for (int i = 0; i < 3; ++i) {
+            if (i == 2 && !(P_SPLIT && few)) break;
+            if constexpr (E == 4)
+              *reinterpret_cast<uint2*>(smem + at + i * next) = make_uint2(term[i][0], term[i][1]);
+            else
+              *reinterpret_cast<uint32_t*>(smem + at + i * next) = term[i][0];
           }
         }
       }
@@ -363,7 +374,7 @@ __global__ void __maxnreg__(kLaunchRegs)
 #pragma unroll
             for (int kk = 0; kk < HD / 16; ++kk)
               tc_mma_ss(tS + w * 128, kd + ((kk >> 2) * 16384 + (kk & 3) * 32) / 16,
-                        qd + ((kk >> 2) * 2048 + (kk & 3) * 32) / 16, idesc_bf16_f32(128, 16, 0, 0), kk > 0);
+                        qd + ((kk >> 2) * S::CHUNK + (kk & 3) * 32) / 16, idesc_bf16_f32(128, P_SPLIT ? 32 : 16, 0, 0), kk > 0);
           } else {
 #pragma unroll 1
             for (int term = 0; term < 2; ++term)
@@ -398,7 +409,7 @@ __global__ void __maxnreg__(kLaunchRegs)
             const uint64_t pd = p0 + w * (S::PT_BYTES >> 4);
 #pragma unroll
             for (int kk = 0; kk < 8; ++kk)
-              tc_mma_ss(oc, vd + kk * 128, pd + ((kk >> 2) * 2048 + (kk & 3) * 32) / 16, idesc_bf16_f32(128, 16, 1, 0),
+              tc_mma_ss(oc, vd + kk * 128, pd + ((kk >> 2) * S::CHUNK + (kk & 3) * 32) / 16, idesc_bf16_f32(128, P_SPLIT ? 32 : 16, 1, 0),
                         t > sg.t0 || kk > 0);
           } else {
 #pragma unroll 1
@@ -423,10 +434,11 @@ __global__ void __maxnreg__(kLaunchRegs)
     bool another = more;
     for (int s = 0; more; ++s) {
       if (another) {
-        // up to 8 rows alternate between two buffers, up to 64 between two halves of one; where more are
-        // involved, the scores before have to be done
+        // up to 8 rows alternate between two buffers, up to 64 between two halves of one that lies over these;
+        // where more are involved, or one form follows the other, what was read from there has to be done
         const int n0 = rows_of(p, sg), n1 = rows_of(p, nx);
-        if (s > 0 && min(n0, n1) > kFew && max(n0, n1) > 64) wait(&sq_done[(s - 1) & 1], (s - 1) >> 1);
+        if (s > 0 && n0 > kFew && (n1 <= kFew || max(n0, n1) > 64)) wait(&sq_done[(s - 1) & 1], (s - 1) >> 1);
+        if (s > 0 && n0 <= kFew && n1 > kFew) wait(&so_full[(s - 1) & 1], (s - 1) >> 1);
         prepare(nx, s, s == 0 ? warp : q, s == 0 ? 12 : 4);
         if (s == 0) named_bar_sync(4, 384);
         if (warp < kWarpQo) break;
@@ -464,12 +476,12 @@ __global__ void __maxnreg__(kLaunchRegs)
           }
         } else {
           if (32 * q < HD) {  // lane l holds element l of every row
-            float v[2 * kFew];
-            tmem_ld16(oc, v);
+            float v[kCols];
+            tmem_ld_cols(oc, v);
             tmem_wait_ld();
 #pragma unroll
             for (int h = 0; h < kFew; ++h)
-              if (h < n) o[h * HD + l] = P_SPLIT ? v[h] + v[kFew + h] : v[h];
+              if (h < n) o[h * HD + l] = P_SPLIT ? v[h] + (v[kFew + h] + v[kCols - 2 * kFew + h]) : v[h];
           }
           if (l < n) ml[l] = make_float2(st[32 + l], (st[l] + st[8 + l]) + (st[16 + l] + st[24 + l]));
         }
@@ -500,11 +512,12 @@ __global__ void __maxnreg__(kLaunchRegs)
           tc_fence_after();
           float x[H];
           {
-            float raw[2 * kFew];
-            tmem_ld16(tS + w * 128 + lane_off, raw);
+            float raw[kCols];
+            tmem_ld_cols(tS + w * 128 + lane_off, raw);
             tmem_wait_ld();
 #pragma unroll
-            for (int h = 0; h < H; ++h) x[h] = j < nk && h < n ? raw[h] + raw[kFew + h] : -INFINITY;
+            for (int h = 0; h < H; ++h)
+              x[h] = j < nk && h < n ? raw[h] + (P_SPLIT ? raw[kFew + h] + raw[kCols - 2 * kFew + h] : raw[kFew + h]) : -INFINITY;
           }
           bool over = t == sg.t0;
           if (t > sg.t0) {
@@ -534,30 +547,34 @@ __global__ void __maxnreg__(kLaunchRegs)
               wait(&o_done[(i - 1) & 1], i - 1 >> 1);
               tc_fence_after();
               const uint32_t o_at = tO + (seg & 1) * 128 + lane_off;
-              float v[2 * kFew];
-              tmem_ld16(o_at, v);
+              float v[kCols];
+              tmem_ld_cols(o_at, v);
               tmem_wait_ld();
 #pragma unroll
               for (int h = 0; h < H; ++h) {
                 l[h] *= a_s[h];
-                v[h] *= a_s[h];
-                v[kFew + h] *= a_s[h];
+#pragma unroll
+                for (int i = 0; i < kCols; i += kFew) v[i + h] *= a_s[h];
               }
               tmem_st_cols(o_at, v);
               tmem_wait_st();
               tc_fence_before();
             }
           }
-          uint8_t* Pt = smem + S::OFF_PT + w * S::PT_BYTES + (j >> 6) * 2048 + (j & 7) * 2;
+          uint8_t* Pt = smem + S::OFF_PT + w * S::PT_BYTES + (j >> 6) * S::CHUNK + (j & 7) * 2;
           const int unit = (j & 63) >> 3;
 #pragma unroll
           for (int h = 0; h < H; ++h) {
-            const float top = m_s[h], y = ex2_approx(x[h] - (top == -INFINITY ? 0.f : top));
+            const float top = m_s[h];
+            float y = ex2_approx(x[h] - (top == -INFINITY ? 0.f : top));
             l[h] += y;
-            const __nv_bfloat16 b = __float2bfloat16_rn(y);
-            const int at = h * 128 + ((unit ^ h) << 4);
-            *reinterpret_cast<__nv_bfloat16*>(Pt + at) = b;
-            if (P_SPLIT) *reinterpret_cast<__nv_bfloat16*>(Pt + at + kFew * 128) = __float2bfloat16_rn(y - __bfloat162float(b));
+            uint8_t* at = Pt + h * 128 + ((unit ^ h) << 4);
+#pragma unroll
+            for (int i = 0; i < (P_SPLIT ? 3 : 1); ++i) {
+              const __nv_bfloat16 b = __float2bfloat16_rn(y);
+              *reinterpret_cast<__nv_bfloat16*>(at + i * kFew * 128) = b;
+              y -= __bfloat162float(b);
+            }
           }
           if (nk < CutTc::KT && !sg.prefix) {
             // rows past the request's last: P is zero there, but what the cache holds may be NaN (past a
