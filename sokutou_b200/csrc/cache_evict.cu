@@ -184,8 +184,9 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const Params p) {
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
       const int eb = e + __popc(be[i] & below);
-      if (((bs[i] >> lane) & 1) || (((be[i] >> lane) & 1) && eb < room))
-        list[s + __popc(bs[i] & below) + min(eb, room)] = block * BLOCK + j0 + 32 * i;
+      const int at = s + __popc(bs[i] & below) + min(eb, room);
+      if ((((bs[i] >> lane) & 1) || (((be[i] >> lane) & 1) && eb < room)) && SK_INB(at < p.keep, p.err))
+        list[at] = block * BLOCK + j0 + 32 * i;
       s += __popc(bs[i]);
       e += __popc(be[i]);
     }
@@ -225,7 +226,7 @@ __global__ void __launch_bounds__(kMoveThreads) move_in_place_kernel(const Param
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       const int d = d0 + i * RPP + t / U;
-      if (src[i] != d) v[i] = *reinterpret_cast<const uint4*>(base + src[i] * p.kv[3]);
+      if (src[i] != d && SK_INB(src[i] > d && src[i] < n, p.err)) v[i] = *reinterpret_cast<const uint4*>(base + src[i] * p.kv[3]);
     }
     __syncthreads();
 #pragma unroll
@@ -280,7 +281,10 @@ __global__ void __launch_bounds__(kMoveThreads, 6) move_copy_kernel(const Params
 #pragma unroll
     for (int b = 0; b < kCopyBatch; ++b) {
       const int x = d + b * RPP;
-      if (x < d1) v[b] = __ldcs(reinterpret_cast<const uint4*>(src + (all ? x : __ldg(list + x)) * p.kv[3]));
+      if (x < d1) {
+        const int from = all ? x : __ldg(list + x);
+        if (SK_INB(from >= x && from < n, p.err)) v[b] = __ldcs(reinterpret_cast<const uint4*>(src + from * p.kv[3]));
+      }
     }
 #pragma unroll
     for (int b = 0; b < kCopyBatch; ++b) {

@@ -185,6 +185,7 @@ __global__ void __launch_bounds__(kSimtThreads) tiles_simt_kernel(const Params p
       }
     }
     const long long slot = (long long)c + sg.item;
+    if (!SK_INB(slot < (sg.prefix ? p.slots_p : p.slots_o), p.err)) return;
     float* o = sg.prefix ? p.po + slot * RT * HD : p.oo + slot * p.g * HD;
     float* ml = sg.prefix ? p.pml + slot * RT * 2 : p.oml + slot * p.g * 2;
 #pragma unroll
@@ -316,7 +317,7 @@ __global__ void __launch_bounds__(kJoinThreads, 5) join_kernel(const Params p) {
       for (int b = 0; b < kAhead; ++b) {
         const int x = x0 + b * per;
         ml[b] = make_float2(-INFINITY, 0.f);
-        if (x < np + no) {
+        if (x < np + no && SK_INB(x < np ? pc + x + ip < p.slots_p : oc + x - np + io < p.slots_o, p.err)) {
           const long long at = x < np ? (long long)(pc + x + ip) * RT + il : (long long)(oc + x - np + io) * p.g + h;
           ml[b] = __ldcg(reinterpret_cast<const float2*>(x < np ? p.pml : p.oml) + at);
           if (blockIdx.y == 0) load_vec_cg<E>((x < np ? p.po : p.oo) + at * HD + lane * E, o[b]);
@@ -532,6 +533,7 @@ extern "C" int sk_decode_attention_shared(const SkSharedDecode* d, const void* q
   p.po = reinterpret_cast<float*>(ws + w.po), p.pml = reinterpret_cast<float*>(ws + w.pml);
   p.oo = reinterpret_cast<float*>(ws + w.oo), p.oml = reinterpret_cast<float*>(ws + w.oml);
   p.sc = reinterpret_cast<float*>(ws + w.sc), p.sc_stride = w.sc_stride;
+  p.slots_p = (int)w.slots_p, p.slots_o = (int)w.slots_o;
   p.err = sk_error_word_ptr();
   if (!p.err) return SK_ERR_CUDA;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);

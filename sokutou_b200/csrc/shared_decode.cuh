@@ -69,6 +69,7 @@ struct Params {
   float* oml;
   float* sc;           // log2-domain scores of the own rows [R][nq][sc_stride] (mass only)
   long long sc_stride;
+  int slots_p, slots_o;  // partials that the workspace holds (bounds-checked build)
   int* err;
 };
 
@@ -90,13 +91,14 @@ __host__ inline bool too_many_tiles(long long R, long long g, long long nkv, lon
 __host__ __device__ inline long long align_up(long long x, long long a) { return (x + a - 1) / a * a; }
 
 struct WsLayout {
-  long long po, pml, oo, oml, sc, sc_stride, bytes;
+  long long po, pml, oo, oml, sc, sc_stride, bytes, slots_p, slots_o;
 };
 template <class Cut>
 __host__ inline WsLayout ws_layout(int R, int nq, int nkv, int hd, int P, int max_len, bool mass) {
   const long long g = nq / nkv, items_p = P > 0 ? (long long)nkv * ((R * g + Cut::RT - 1) / Cut::RT) : 0;
   const long long slots_p = P > 0 ? items_p + Cut::G : 0, slots_o = (long long)R * nkv + Cut::G;
   WsLayout w;
+  w.slots_p = slots_p, w.slots_o = slots_o;
   long long at = 0;
   auto take = [&](long long n) {
     const long long p = at;

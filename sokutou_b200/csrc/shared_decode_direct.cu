@@ -118,6 +118,7 @@ __device__ __forceinline__ void finish(const Params& p, bool clustered, int clus
       o += a * part[c];
     }
     const long long at = r * p.out_stride + (long long)kvh * g * HD + x;
+    if (!SK_INB(kvh * g * HD + x < p.nq * HD, p.err)) continue;
     if (p.out_bf16)
       reinterpret_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(o / L);
     else
@@ -161,7 +162,7 @@ __device__ __forceinline__ void finish(const Params& p, bool clustered, int clus
 #pragma unroll
       for (int i = 0; i < kAtOnce; ++i) {
         const int j = j0 + i * kThreads;
-        if (j < jb) mass[j] = before[i] + sum[i];
+        if (j < jb && SK_INB(j < p.max_len, p.err)) mass[j] = before[i] + sum[i];
       }
     }
   }
@@ -345,7 +346,7 @@ __global__ void __launch_bounds__(kMmaThreads, MmaSmem<HD, THIRD>::kPerSm) direc
     uint8_t* at = smem + w * NST * S::SLOT + slot * S::SLOT;
     const bool own = b >= nbp;
     const int j0 = (own ? b - nbp : b) * kRows, valid = own ? n + 1 - j0 : p.P - j0;  // rows, if fewer than 16
-    if (b == nb - 1) {  // the new row in its place
+    if (b == nb - 1 && SK_INB(n - j0 >= 0 && n - j0 < kRows, p.err)) {  // the new row in its place
       uint8_t* dst = at + (n - j0) * S::PITCH;
       for (int x = lane; x < 2 * U; x += 32)
         *reinterpret_cast<uint4*>(dst + (x / U) * S::HALF + (x % U) * 16) = *reinterpret_cast<const uint4*>(new_s + x * 16);
@@ -383,7 +384,7 @@ __global__ void __launch_bounds__(kMmaThreads, MmaSmem<HD, THIRD>::kPerSm) direc
         if (THIRD == kInRows) x += __shfl_xor_sync(0xffffffffu, x, 16);  // rows h and 4 + h
         s[u][e] = j < valid ? x : -INFINITY;
         over |= h < g && s[u][e] > m + 8.0f;
-        if (sc && own && j < valid) sc[j0 + j] = s[u][e];
+        if (sc && own && j < valid && SK_INB(j0 + j < p.max_len, p.err)) sc[j0 + j] = s[u][e];
       }
     if (__any_sync(0xffffffffu, over)) {
       float t = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));

@@ -449,7 +449,8 @@ __global__ void __maxnreg__(kLaunchRegs)
         wait(&so_full[seg & 1], seg >> 1);
         wait(&ml_full[seg & 1], seg >> 1);
         tc_fence_after();
-        const long long slot = (long long)c + sg.item;
+        long long slot = (long long)c + sg.item;
+        if (!SK_INB(slot < (sg.prefix ? p.slots_p : p.slots_o), p.err)) slot = 0;
         const long long row0 = sg.prefix ? slot * CutTc::RT : slot * p.g;  // first partial row
         float* o = (sg.prefix ? p.po : p.oo) + row0 * HD;
         float2* ml = reinterpret_cast<float2*>(sg.prefix ? p.pml : p.oml) + row0;
@@ -527,7 +528,7 @@ __global__ void __maxnreg__(kLaunchRegs)
           if (sc) {
 #pragma unroll
             for (int h = 0; h < H; ++h)
-              if (h < n) sc[h * p.sc_stride + (long long)t * CutTc::KT] = x[h];
+              if (h < n && SK_INB(t * CutTc::KT + j < p.sc_stride, p.err)) sc[h * p.sc_stride + (long long)t * CutTc::KT] = x[h];
           }
           if (any_of_128(over)) {
             float y[H];
