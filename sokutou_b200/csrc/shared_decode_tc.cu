@@ -57,20 +57,22 @@ struct MapOrder {
   int row, head, req;  // 0..2: dimension 1 + that
 };
 
-template <int HD>
+template <int HD, bool P_SPLIT>
 struct SmemTc {
   static constexpr int NSK = HD == 128 ? 2 : 4, NSV = HD == 128 ? 2 : 4;
   static constexpr int NCH = HD / 64;
   static constexpr int Q_BYTES = 128 * HD * 2, KV_BYTES = 128 * HD * 2;
-  // Query area. n > 8: hi rows, then lo rows [128][hd], 64-element chunks 16 KB apart. n <= 8: two buffers of 24
-  // rows (8 of each term) and two of P^T [24 rows][128 keys], 64-element chunks 3 KB apart; a product reads 32
-  // rows, the last 8 whatever comes next, for columns that are not used.
-  static constexpr int OFF_Q = 0, CHUNK = 24 * 128;
+  // Query area. n > 8: hi rows, then lo rows [128][hd], 64-element chunks 16 KB apart. n <= 8: two buffers of 8
+  // rows of each term and two of P^T [as many][128 keys]; two terms behind the first area, three (P_SPLIT), for
+  // which there is no room, over it (a product then reads 32 rows, the last 8 whatever comes next, for columns
+  // that are not used).
+  static constexpr bool kOver = P_SPLIT;
+  static constexpr int OFF_Q = 0, CHUNK = (P_SPLIT ? 24 : 16) * 128;  // bytes per 64 elements
   static constexpr int QT_BYTES = NCH * CHUNK, PT_BYTES = 2 * CHUNK;
-  static constexpr int OFF_QT = OFF_Q, OFF_PT = OFF_QT + 2 * QT_BYTES;
-  static_assert(OFF_PT + 2 * PT_BYTES + 1024 <= 2 * Q_BYTES, "the query area holds either form");
+  static constexpr int OFF_QT = kOver ? OFF_Q : OFF_Q + 2 * Q_BYTES, OFF_PT = OFF_QT + 2 * QT_BYTES;
+  static_assert(!kOver || OFF_PT + 2 * PT_BYTES + 1024 <= 2 * Q_BYTES, "the query area holds either form");
   // V before K: at hd = 64 the V^T operand (M = 128) reads 16 KB past its tile, into lanes that are not used
-  static constexpr int OFF_V = OFF_Q + 2 * Q_BYTES;
+  static constexpr int OFF_V = kOver ? OFF_Q + 2 * Q_BYTES : OFF_PT + 2 * PT_BYTES;
   static constexpr int OFF_K = OFF_V + NSV * KV_BYTES;
   static constexpr int OFF_ML = OFF_K + NSK * KV_BYTES;  // [2] n > 8: [128] (max, sum of A), [128] sum of B;
   static constexpr int ML_FLOATS = 3 * 128;              //     n <= 8: sums [4][8], max [8]
@@ -187,7 +189,7 @@ __global__ void __maxnreg__(kLaunchRegs)
     tiles_tc_kernel(const __grid_constant__ CUtensorMap tmKp, const __grid_constant__ CUtensorMap tmVp,
                     const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                     const __grid_constant__ TcArgs args) {
-  using S = SmemTc<HD>;
+  using S = SmemTc<HD, P_SPLIT>;
   constexpr int NSK = S::NSK, NSV = S::NSV, NCH = S::NCH, E = HD / 32;
   constexpr int kCols = P_SPLIT ? 32 : 16;  // columns of the products of few rows: 8 per term, 8 more to the next 16
   const Params& p = args.p;
@@ -267,6 +269,16 @@ __global__ void __maxnreg__(kLaunchRegs)
     const bool few = n <= kFew;
     constexpr int kRowsAhead = 4;
     const int base = few ? 0 : base_of(n, seg);
+    if (n > step * kRowsAhead) {  // several batches: start all rows' trip to L2 now, lines of four rows at a time
+      for (int i = first + step * (lane >> 3); i < n; i += 4 * step) {
+        const int row = s.r * CutTc::RT + i, r = (int)((uint32_t)row / p.g), line = lane & 3;
+        const char* at = reinterpret_cast<const char*>(p.rope + (long long)ls.pos[r] * HD);
+        if (lane & 4)
+          at = reinterpret_cast<const char*>(p.qkv) + (r * p.qkv_stride + (long long)(s.kvh * p.g + row - r * p.g) * HD) * (p.qkv_bf16 ? 2 : 4);
+        if (line * 128 < HD * ((lane & 4) && p.qkv_bf16 ? 2 : 4))
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(at + line * 128));
+      }
+    }
 #pragma unroll 1
     for (int i0 = first; i0 < n; i0 += step * kRowsAhead) {
       RawRow<HD> raw[kRowsAhead];
@@ -300,7 +312,7 @@ __global__ void __maxnreg__(kLaunchRegs)
         const int in_row = (base + i) * 128 + ((unit ^ (i & 7)) << 4) + (d & 7) * 2;
         const int at = few ? S::OFF_QT + (seg & 1) * S::QT_BYTES + chunk * S::CHUNK + in_row : S::OFF_Q + chunk * 16384 + in_row;
         const int next = few ? kFew * 128 : S::Q_BYTES;  // from one term to the next
-        if (SK_INB(at + next + 2 * E <= 2 * S::Q_BYTES, p.err)) {
+        if (SK_INB(at + next + 2 * E <= (few ? S::OFF_PT : 2 * S::Q_BYTES), p.err)) {
 #pragma unroll
           for (int i = 0; i < 3; ++i) {
             if (i == 2 && !(P_SPLIT && few)) break;
@@ -434,11 +446,11 @@ __global__ void __maxnreg__(kLaunchRegs)
     bool another = more;
     for (int s = 0; more; ++s) {
       if (another) {
-        // up to 8 rows alternate between two buffers, up to 64 between two halves of one that lies over these;
-        // where more are involved, or one form follows the other, what was read from there has to be done
+        // up to 8 rows alternate between two buffers, up to 64 between two halves of one; where more are involved,
+        // or one form follows the other in the same place, what was read from there has to be done
         const int n0 = rows_of(p, sg), n1 = rows_of(p, nx);
-        if (s > 0 && n0 > kFew && (n1 <= kFew || max(n0, n1) > 64)) wait(&sq_done[(s - 1) & 1], (s - 1) >> 1);
-        if (s > 0 && n0 <= kFew && n1 > kFew) wait(&so_full[(s - 1) & 1], (s - 1) >> 1);
+        if (s > 0 && n0 > kFew && (n1 <= kFew ? S::kOver : max(n0, n1) > 64)) wait(&sq_done[(s - 1) & 1], (s - 1) >> 1);
+        if (s > 0 && n0 <= kFew && n1 > kFew && S::kOver) wait(&so_full[(s - 1) & 1], (s - 1) >> 1);
         prepare(nx, s, s == 0 ? warp : q, s == 0 ? 12 : 4);
         if (s == 0) named_bar_sync(4, 384);
         if (warp < kWarpQo) break;
@@ -769,7 +781,7 @@ static int launch(const Params& p, cudaStream_t st) {
     kp = k;  // never read
     vp = v;
   }
-  const int smem = SmemTc<HD>::bytes(p.R);
+  const int smem = SmemTc<HD, P_SPLIT>::bytes(p.R);
   if (cudaFuncSetAttribute(tiles_tc_kernel<HD, P_SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
       cudaSuccess)
     return SK_ERR_CUDA;
