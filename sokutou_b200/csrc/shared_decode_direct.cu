@@ -193,6 +193,17 @@ __device__ __forceinline__ void split(float a, float b, uint32_t (&x)[N]) {
     b -= __uint_as_float(x[i] & 0xffff0000u);
   }
 }
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&d)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {  // 16-bit elements, row lane / 4, columns 2 (lane % 4), + 1
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&d)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
@@ -205,9 +216,10 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool k
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(keep ? 16 : 0) : "memory");
 }
 
-// How q's third term is taken: not at all (bf16 out and no weights kept, which two terms are exact enough for),
-// in rows of the product that four heads leave free, or in products of its own.
-enum Third { kNoThird, kInRows, kApart };
+// How q's third term is taken with more than two heads: not at all (bf16 out and no weights kept, which two terms
+// are exact enough for), in rows of the product that four heads leave free, or in products of its own. kByKeys, up to
+// two heads: the keys and the elements are the products' rows, the terms of both heads its eight columns.
+enum Third { kNoThird, kInRows, kApart, kByKeys };
 
 template <int HD, Third THIRD>
 struct MmaSmem {
@@ -217,7 +229,7 @@ struct MmaSmem {
   static constexpr int NST = HD == 128 ? 3 : 4, kPerSm = HD == 128 || THIRD == kApart ? 2 : 3;
   static constexpr int PITCH = HD * 2 + 16;       // bytes: an odd number of 16-byte units, no bank conflicts
   static constexpr int HALF = kRows * PITCH, SLOT = 2 * HALF;  // K, V
-  static constexpr int kTerms = THIRD == kApart ? 3 : 2;
+  static constexpr int kTerms = THIRD == kApart ? 3 : THIRD == kByKeys ? 1 : 2;
   static constexpr int OFF_Q = kMmaWarps * NST * SLOT;                // [kTerms][8 rows][PITCH]: see the kernel
   static constexpr int OFF_NEW = OFF_Q + kTerms * kMaxGroup * PITCH;  // the new token's k and v
   static constexpr int BYTES = OFF_NEW + 2 * HD * 2;
@@ -289,10 +301,11 @@ __global__ void __launch_bounds__(kMmaThreads, MmaSmem<HD, THIRD>::kPerSm) direc
   // q, and the new token's k and v
   // The product's rows 0-7 and 8-15 are q_s[0] and q_s[1]: head h's first term in row h, its second in row 8 + h,
   // its third in row 4 + h (kInRows) or in q_s[2] (kApart); the rows left over are zero.
+  // kByKeys: head h's term i in row 2 i + h of q_s[0], the columns of the product.
   constexpr int kTerms = THIRD == kNoThird ? 2 : 3;
   for (int x = w; x < S::kTerms * GP; x += kMmaWarps) {
     const int y = x % GP;
-    const bool used = y < g || (THIRD == kInRows && x < GP && y >= 4 && y < 4 + g);
+    const bool used = THIRD == kByKeys ? y < 6 && y % 2 < g : y < g || (THIRD == kInRows && x < GP && y >= 4 && y < 4 + g);
     if (!used && lane < U) *reinterpret_cast<uint4*>(smem + S::OFF_Q + x * S::PITCH + lane * 16) = make_uint4(0, 0, 0, 0);
   }
   for (int x = w; x < g + 2; x += kMmaWarps) {
@@ -310,6 +323,11 @@ __global__ void __launch_bounds__(kMmaThreads, MmaSmem<HD, THIRD>::kPerSm) direc
         uint32_t term[kTerms];
         split(y[0][e] * p.q_scale, y[0][e + 1] * p.q_scale, term);
         uint8_t* dst = smem + S::OFF_Q + (lane * EL + e) * 2;
+        if (THIRD == kByKeys) {
+#pragma unroll
+          for (int i = 0; i < kTerms; ++i) *reinterpret_cast<uint32_t*>(dst + (2 * i + x) * S::PITCH) = term[i];
+          continue;
+        }
         *reinterpret_cast<uint32_t*>(dst + x * S::PITCH) = term[0];
         *reinterpret_cast<uint32_t*>(dst + (GP + x) * S::PITCH) = term[1];
         if (THIRD != kNoThird)
@@ -327,119 +345,228 @@ __global__ void __launch_bounds__(kMmaThreads, MmaSmem<HD, THIRD>::kPerSm) direc
   }
   __syncthreads();
 
-  const int h = THIRD == kInRows ? row & 3 : row;  // this lane's head (rows 4-7 keep step with 0-3)
-  float m = -INFINITY, l = 0.f;  // of head h, the same in its four lanes / this lane's part
-  float o[HD / 8][4];            // elements 8 t + 2c, + 1 by the weights' first (or third) terms, then by their second
-#pragma unroll
-  for (int t = 0; t < HD / 8; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
-  float* sc = p.mass && row < g ? p.sc + ((long long)r * p.nq + kvh * g + row) * p.sc_stride : nullptr;
-  const uint8_t* q_at = smem + S::OFF_Q + row * S::PITCH + 16 * c;
-  // ldmatrix: lane x gives the row of matrix x / 8: keys x % 8 (+ 8 for the odd ones), 8 elements on for 2 and 3
-  const uint32_t v_at = S::HALF + (lane & 15) * S::PITCH + (lane >> 4) * 16;
-
   int slot = 0;
-#pragma unroll 1
-  for (int b = b0 + w; b < b1; b += kMmaWarps) {
+  // The next batch of this warp: waits for its copies, starts those of a later one, puts the new row in its place.
+  const auto next_batch = [&](int b, int& j0, int& valid, bool& own) __attribute__((always_inline)) -> uint8_t* {
     asm volatile("cp.async.wait_group %0;" ::"n"(NST - 2) : "memory");
     __syncwarp();  // this batch has landed for every lane, and every lane is past the one whose slot is next
     fetch(b + (NST - 1) * kMmaWarps, slot == 0 ? NST - 1 : slot - 1);
     uint8_t* at = smem + w * NST * S::SLOT + slot * S::SLOT;
-    const bool own = b >= nbp;
-    const int j0 = (own ? b - nbp : b) * kRows, valid = own ? n + 1 - j0 : p.P - j0;  // rows, if fewer than 16
-    if (b == nb - 1 && SK_INB(n - j0 >= 0 && n - j0 < kRows, p.err)) {  // the new row in its place
+    own = b >= nbp;
+    j0 = (own ? b - nbp : b) * kRows;
+    valid = own ? n + 1 - j0 : p.P - j0;  // rows, if fewer than 16
+    if (b == nb - 1 && SK_INB(n - j0 >= 0 && n - j0 < kRows, p.err)) {
       uint8_t* dst = at + (n - j0) * S::PITCH;
       for (int x = lane; x < 2 * U; x += 32)
         *reinterpret_cast<uint4*>(dst + (x / U) * S::HALF + (x % U) * 16) = *reinterpret_cast<const uint4*>(new_s + x * 16);
       __syncwarp();
     }
-    const uint8_t* k_at = at + row * S::PITCH + 16 * c;
-    float s[2][4], s2[2][4];  // two chains of products each
+    return at;
+  };
+  if constexpr (THIRD == kByKeys) {
+    // S^T = K·Q^T: a lane has keys row and row + 8, columns 2c, 2c + 1 = both heads' term c; O^T = V^T·P^T: elements
+    // row and row + 8 of 16, the same columns. Half the products of the other form, which has 8 heads' rows to fill.
+    uint32_t q[HD / 16][2];  // right operand
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int i = 0; i < HD / 16; i += 2) {
+      uint32_t x[4];
+      ldmatrix_x4(x, smem_u32(smem) + S::OFF_Q + (lane & 7) * S::PITCH + (lane >> 3) * 16 + i * 32);
+      q[i][0] = x[0], q[i][1] = x[1], q[i + 1][0] = x[2], q[i + 1][1] = x[3];
+    }
+    // ldmatrix: lane x gives a row of matrix x / 8. K: keys x % 16, elements + 8 for matrices 2, 3; V: keys x % 8, + 8
+    // for matrices 2, 3, elements + 8 for 1, 3
+    const uint32_t k_at = (lane & 15) * S::PITCH + (lane >> 4) * 16;
+    const uint32_t v_at = S::HALF + ((lane & 7) + ((lane >> 4) << 3)) * S::PITCH + ((lane >> 3) & 1) * 16;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {};  // of the heads; l: of this lane's keys
+    float o[HD / 16][4];                             // head 0, 1 of element row, of row + 8
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[u][e] = s2[u][e] = 0.f;
+    for (int t = 0; t < HD / 16; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
+    float* sc = p.mass && c < g ? p.sc + ((long long)r * p.nq + kvh * g + c) * p.sc_stride : nullptr;
+#pragma unroll 1
+    for (int b = b0 + w; b < b1; b += kMmaWarps) {
+      int j0, valid;
+      bool own;
+      const uint32_t at = smem_u32(next_batch(b, j0, valid, own));
+      float d[2][4] = {};  // two chains of products
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const uint4 hi = *reinterpret_cast<const uint4*>(q_at + 64 * i);
-      const uint4 lo = *reinterpret_cast<const uint4*>(q_at + GP * S::PITCH + 64 * i);
+      for (int i = 0; i < HD / 16; ++i) {
+        uint32_t k[4];
+        ldmatrix_x4(k, at + k_at + i * 32);
+        mma_bf16(d[i & 1], k[0], k[1], k[2], k[3], q[i][0], q[i][1]);
+      }
+      float s[2][2];  // [key row + 8 u][head]
+      bool over = false;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const uint4 k = *reinterpret_cast<const uint4*>(k_at + 8 * u * S::PITCH + 64 * i);
-        mma_bf16(s[u], hi.x, lo.x, hi.y, lo.y, k.x, k.y);
-        mma_bf16(s2[u], hi.z, lo.z, hi.w, lo.w, k.z, k.w);
-        if (THIRD == kApart) {
-          const uint4 third = *reinterpret_cast<const uint4*>(q_at + 2 * GP * S::PITCH + 64 * i);
-          mma_bf16(s[u], third.x, 0, third.y, 0, k.x, k.y);
-          mma_bf16(s2[u], third.z, 0, third.w, 0, k.z, k.w);
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float x = d[0][2 * u + h] + d[1][2 * u + h];
+          x += __shfl_xor_sync(0xffffffffu, x, 1);
+          x += __shfl_xor_sync(0xffffffffu, x, 2);
+          s[u][h] = row + 8 * u < valid && h < g ? x : -INFINITY;
+          over |= s[u][h] > m[h] + 8.0f;
+        }
+      if (sc && own) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          if (row + 8 * u < valid && SK_INB(j0 + row + 8 * u < p.max_len, p.err)) sc[j0 + row + 8 * u] = c == 0 ? s[u][0] : s[u][1];
+      }
+      if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float t = fmaxf(s[0][h], s[1][h]);
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
+          t = fmaxf(t, m[h]);
+          const float a = t == -INFINITY ? 1.f : ex2_approx(m[h] - t);
+          m[h] = t;
+          l[h] *= a;
+#pragma unroll
+          for (int x = 0; x < HD / 16; ++x) o[x][h] *= a, o[x][2 + h] *= a;
         }
       }
-    }
-    bool over = false;
+      uint32_t pb[2];  // right operand: term c of both heads' weights, turned so that keys come in pairs
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int j = 8 * u + 2 * c + e;
-        float x = (s[u][e] + s2[u][e]) + (s[u][2 + e] + s2[u][2 + e]);
-        if (THIRD == kInRows) x += __shfl_xor_sync(0xffffffffu, x, 16);  // rows h and 4 + h
-        s[u][e] = j < valid ? x : -INFINITY;
-        over |= h < g && s[u][e] > m + 8.0f;
-        if (sc && own && j < valid && SK_INB(j0 + j < p.max_len, p.err)) sc[j0 + j] = s[u][e];
+      for (int u = 0; u < 2; ++u) {
+        const float x = ex2_approx(s[u][0] - (m[0] == -INFINITY ? 0.f : m[0]));
+        const float y = ex2_approx(s[u][1] - (m[1] == -INFINITY ? 0.f : m[1]));
+        l[0] += x;
+        l[1] += y;
+        uint32_t term[3];
+        split(x, y, term);
+        pb[u] = transpose_8x8(c == 0 ? term[0] : c == 1 ? term[1] : c == 2 ? term[2] : 0u);
       }
-    if (__any_sync(0xffffffffu, over)) {
-      float t = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
-      t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
-      t = fmaxf(fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2)), m);
-      const float a = t == -INFINITY ? 1.f : ex2_approx(m - t);
-      m = t;
-      l *= a;
 #pragma unroll
-      for (int x = 0; x < HD / 8; ++x)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[x][e] *= a;
-    }
-    const float use = m == -INFINITY ? 0.f : m;
-    // left operand: rows 0-7 for the keys of u = 0, rows 8-15, the same for u = 1; third terms where q's are
-    uint32_t a[4], a3[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const float x = ex2_approx(s[u][0] - use), y = ex2_approx(s[u][1] - use);
-      l += x + y;
-      uint32_t term[kTerms];
-      split(x, y, term);
-      const bool third = THIRD == kInRows && row >= 4;
-      a[2 * u] = third ? term[kTerms - 1] : term[0];
-      a[2 * u + 1] = third ? 0u : term[1];
-      a3[u] = term[kTerms - 1];
-    }
-#pragma unroll
-    for (int t = 0; t < HD / 8; t += 2) {
-      uint32_t vb[4];
-      ldmatrix_x4_trans(vb, ring + slot * S::SLOT + v_at + t * 16);
-      mma_bf16(o[t], a[0], a[1], a[2], a[3], vb[0], vb[1]);
-      mma_bf16(o[t + 1], a[0], a[1], a[2], a[3], vb[2], vb[3]);
-      if (THIRD == kApart) {
-        mma_bf16(o[t], a3[0], 0, a3[1], 0, vb[0], vb[1]);
-        mma_bf16(o[t + 1], a3[0], 0, a3[1], 0, vb[2], vb[3]);
+      for (int t = 0; t < HD / 16; ++t) {
+        uint32_t v[4];
+        ldmatrix_x4_trans(v, at + v_at + t * 32);
+        mma_bf16(o[t], v[0], v[1], v[2], v[3], pb[0], pb[1]);
       }
+      slot = slot == NST - 1 ? 0 : slot + 1;
     }
-    slot = slot == NST - 1 ? 0 : slot + 1;
-  }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], x);
+      if (lane == 0) ml_s[w][h] = make_float2(m[h], l[h]);
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();  // every batch read: the rings take the outputs
+#pragma unroll
+    for (int t = 0; t < HD / 16; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float x = o[t][e];  // the three terms
+        x += __shfl_xor_sync(0xffffffffu, x, 1);
+        x += __shfl_xor_sync(0xffffffffu, x, 2);
+        if (c == e && (e & 1) < g)
+          *reinterpret_cast<float*>(smem + S::OFF_RED + ((w * GP + (e & 1)) * HD + 16 * t + row + 8 * (e >> 1)) * 4) = x;
+      }
+  } else {
+    const int h = THIRD == kInRows ? row & 3 : row;  // this lane's head (rows 4-7 keep step with 0-3)
+    float m = -INFINITY, l = 0.f;  // of head h, the same in its four lanes / this lane's part
+    float o[HD / 8][4];            // elements 8 t + 2c, + 1 by the weights' first (or third) terms, then by their second
+#pragma unroll
+    for (int t = 0; t < HD / 8; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
+    float* sc = p.mass && row < g ? p.sc + ((long long)r * p.nq + kvh * g + row) * p.sc_stride : nullptr;
+    const uint8_t* q_at = smem + S::OFF_Q + row * S::PITCH + 16 * c;
+    // ldmatrix: lane x gives the row of matrix x / 8: keys x % 8 (+ 8 for the odd ones), 8 elements on for 2 and 3
+    const uint32_t v_at = S::HALF + (lane & 15) * S::PITCH + (lane >> 4) * 16;
 
-  l += __shfl_xor_sync(0xffffffffu, l, 1);
-  l += __shfl_xor_sync(0xffffffffu, l, 2);
-  if (c == 0) ml_s[w][row] = make_float2(m, l);  // (rows past g are not read)
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
-  __syncthreads();  // every batch read: the rings take the outputs
+#pragma unroll 1
+    for (int b = b0 + w; b < b1; b += kMmaWarps) {
+      int j0, valid;
+      bool own;
+      const uint8_t* at = next_batch(b, j0, valid, own);
+      const uint8_t* k_at = at + row * S::PITCH + 16 * c;
+      float s[2][4], s2[2][4];  // two chains of products each
 #pragma unroll
-  for (int t = 0; t < HD / 8; ++t) {
-    float x = o[t][0] + o[t][2], y = o[t][1] + o[t][3];
-    if (THIRD == kInRows) {  // row 4 + h
-      x += __shfl_xor_sync(0xffffffffu, x, 16);
-      y += __shfl_xor_sync(0xffffffffu, y, 16);
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[u][e] = s2[u][e] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const uint4 hi = *reinterpret_cast<const uint4*>(q_at + 64 * i);
+        const uint4 lo = *reinterpret_cast<const uint4*>(q_at + GP * S::PITCH + 64 * i);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const uint4 k = *reinterpret_cast<const uint4*>(k_at + 8 * u * S::PITCH + 64 * i);
+          mma_bf16(s[u], hi.x, lo.x, hi.y, lo.y, k.x, k.y);
+          mma_bf16(s2[u], hi.z, lo.z, hi.w, lo.w, k.z, k.w);
+          if (THIRD == kApart) {
+            const uint4 third = *reinterpret_cast<const uint4*>(q_at + 2 * GP * S::PITCH + 64 * i);
+            mma_bf16(s[u], third.x, 0, third.y, 0, k.x, k.y);
+            mma_bf16(s2[u], third.z, 0, third.w, 0, k.z, k.w);
+          }
+        }
+      }
+      bool over = false;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int j = 8 * u + 2 * c + e;
+          float x = (s[u][e] + s2[u][e]) + (s[u][2 + e] + s2[u][2 + e]);
+          if (THIRD == kInRows) x += __shfl_xor_sync(0xffffffffu, x, 16);  // rows h and 4 + h
+          s[u][e] = j < valid ? x : -INFINITY;
+          over |= h < g && s[u][e] > m + 8.0f;
+          if (sc && own && j < valid && SK_INB(j0 + j < p.max_len, p.err)) sc[j0 + j] = s[u][e];
+        }
+      if (__any_sync(0xffffffffu, over)) {
+        float t = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
+        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+        t = fmaxf(fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2)), m);
+        const float a = t == -INFINITY ? 1.f : ex2_approx(m - t);
+        m = t;
+        l *= a;
+#pragma unroll
+        for (int x = 0; x < HD / 8; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[x][e] *= a;
+      }
+      const float use = m == -INFINITY ? 0.f : m;
+      // left operand: rows 0-7 for the keys of u = 0, rows 8-15, the same for u = 1; third terms where q's are
+      uint32_t a[4], a3[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const float x = ex2_approx(s[u][0] - use), y = ex2_approx(s[u][1] - use);
+        l += x + y;
+        uint32_t term[kTerms];
+        split(x, y, term);
+        const bool third = THIRD == kInRows && row >= 4;
+        a[2 * u] = third ? term[kTerms - 1] : term[0];
+        a[2 * u + 1] = third ? 0u : term[1];
+        a3[u] = term[kTerms - 1];
+      }
+#pragma unroll
+      for (int t = 0; t < HD / 8; t += 2) {
+        uint32_t vb[4];
+        ldmatrix_x4_trans(vb, ring + slot * S::SLOT + v_at + t * 16);
+        mma_bf16(o[t], a[0], a[1], a[2], a[3], vb[0], vb[1]);
+        mma_bf16(o[t + 1], a[0], a[1], a[2], a[3], vb[2], vb[3]);
+        if (THIRD == kApart) {
+          mma_bf16(o[t], a3[0], 0, a3[1], 0, vb[0], vb[1]);
+          mma_bf16(o[t + 1], a3[0], 0, a3[1], 0, vb[2], vb[3]);
+        }
+      }
+      slot = slot == NST - 1 ? 0 : slot + 1;
     }
-    if (row < g)
-      *reinterpret_cast<float2*>(smem + S::OFF_RED + (((w * GP + row) * HD) + 8 * t + 2 * c) * 4) = make_float2(x, y);
+
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    if (c == 0) ml_s[w][row] = make_float2(m, l);  // (rows past g are not read)
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();  // every batch read: the rings take the outputs
+#pragma unroll
+    for (int t = 0; t < HD / 8; ++t) {
+      float x = o[t][0] + o[t][2], y = o[t][1] + o[t][3];
+      if (THIRD == kInRows) {  // row 4 + h
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        y += __shfl_xor_sync(0xffffffffu, y, 16);
+      }
+      if (row < g)
+        *reinterpret_cast<float2*>(smem + S::OFF_RED + (((w * GP + row) * HD) + 8 * t + 2 * c) * 4) = make_float2(x, y);
+    }
   }
   finish<GP, HD, kMmaWarps, kMmaThreads>(p, cluster > 1, active, rank, r, kvh, n, max(0, b0 - nbp) * kRows, min(n + 1, (b1 - nbp) * kRows),
                                          &ml_s[0][0], reinterpret_cast<const float*>(smem + S::OFF_RED),
@@ -718,7 +845,7 @@ int launch_direct(const Params& p, int hd, cudaStream_t st) {
   // length, so that long requests get more CTAs than short ones, took longer: 19 to 29 us for 16 slots of 1 to
   // 1404 rows against 18, clusters of which most CTAs leave at once being slow to start.)
   const int per = p.f32 ? (hd == 128 ? 4 : 8) : 16, warps = p.f32 ? kDirWarps : kMmaWarps;
-  const Third third = p.out_bf16 && !p.mass ? kNoThird : p.g <= 4 ? kInRows : kApart;
+  const Third third = p.g <= 2 ? kByKeys : p.out_bf16 && !p.mass ? kNoThird : p.g <= 4 ? kInRows : kApart;
   const int slots = 148 * (p.f32 || hd == 128 || third == kApart ? 2 : MmaSmem<64, kInRows>::kPerSm);
   const long long heads = (long long)p.R * p.nkv, most = (p.P + per - 1) / per + p.max_len / per + 1;  // batches
   int cluster = 1;
@@ -731,7 +858,8 @@ int launch_direct(const Params& p, int hd, cudaStream_t st) {
     return launch(direct_mma_kernel<HD, THIRD>, kMmaThreads, MmaSmem<HD, THIRD>::BYTES, p, cluster, st);
   };
   const auto pick = [&](auto wide) {
-    return third == kNoThird  ? run(wide, std::integral_constant<Third, kNoThird>())
+    return third == kByKeys   ? run(wide, std::integral_constant<Third, kByKeys>())
+           : third == kNoThird ? run(wide, std::integral_constant<Third, kNoThird>())
            : third == kInRows ? run(wide, std::integral_constant<Third, kInRows>())
                               : run(wide, std::integral_constant<Third, kApart>());
   };
