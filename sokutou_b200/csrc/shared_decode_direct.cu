@@ -5,14 +5,17 @@
 // running maximum is a warp's and moves only when a score exceeds it by 2^8.
 //
 // bf16 caches: every warp copies its own batches of 16 keys (8 KB) to shared memory, two ahead of the one that it
-// works on, with the warp-wide tensor instruction (mma.m16n8k16): its 16 rows are the 8 query heads of a group
-// twice, q's first bf16 terms and its second, so a thread gets the two parts of a score in its own registers, and
-// the weights take the same places as the left operand of the value product. Two terms leave out 2^-16 of a
-// number at most; where fp32 goes out or weights are kept both have a third (2^-24), in rows that up to four heads
-// leave free. The inner index of a product may run over the elements in any order, so K is read 16 bytes a lane
-// as it lies and q laid out to match. 16 keys take some 150 instructions; multiplied element by element they took a thousand, and straight from global
-// memory to registers the loads in flight were too few (16 slots behind 96 rows, 1404 rows the longest: 18.7 us so,
-// 18.5 and 23.7 the other ways; one stream of 1119 rows with its weights: 8.6, 9.4 and 9.5 us).
+// works on, with the warp-wide tensor instruction (mma.m16n8k16). Two bf16 terms of a number leave out 2^-16 of it
+// at most; where fp32 goes out or weights are kept, q and the weights have a third (2^-24). Up to two heads: the
+// keys (in the value product the elements) are the product's 16 rows, three terms of both heads its columns, and
+// every term comes with that one product. More heads: its 16 rows are the 8 query heads of a group twice, q's first
+// terms and its second, so a thread gets the two parts of a score in its own registers, and the weights take the
+// same places as the left operand of the value product; the third terms are in rows that up to four heads leave free.
+// The inner index of a product may run over the elements in any order, so there K is read 16 bytes a lane as it
+// lies and q laid out to match. 16 keys take some 150 instructions; multiplied element by element they took a
+// thousand, and straight from global memory to registers the loads in flight were too few (16 slots behind 96 rows,
+// 1404 rows the longest: 18.7 us so, 18.5 and 23.7 the other ways; one stream of 1119 rows with its weights: 8.6,
+// 9.4 and 9.5 us). Two heads in the form for eight: 19.8 and 8.9 us, against 19.2 and 8.7.
 //
 // fp32 caches: element by element; a row takes 16 or 32 lanes, every lane multiplies its elements for all
 // heads, one butterfly leaves each sum in one lane, which exponentiates it, and shuffles bring the weights back.

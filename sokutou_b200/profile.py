@@ -3,6 +3,7 @@
     python -m sokutou_b200.profile --case dit_c1_L512_b3 [--reps 50] [--graph]
     python -m sokutou_b200.profile --case decode_T1120 [--reps 50] [--graph]
     python -m sokutou_b200.profile --case block_T1120 [--reps 50] [--graph]
+    python -m sokutou_b200.profile --case shared_R64_P8192 [--reps 50] [--graph]
 
 Prints one JSON record: the case's shape, average microseconds per call from CUDA events over `reps`
 back-to-back calls (eager launches, or one CUDA graph holding them with --graph), the algorithmic work
@@ -48,6 +49,11 @@ CASES = {
     "block_T1120": ("block", 1120, 2048), "block_T128": ("block", 128, 2048),
     # R independent decode requests in one launch
     "grouped_R8_T1120": ("grouped", 1120, 8), "grouped_R32_T1120": ("grouped", 1120, 32),
+    # R requests of T own rows behind one prefix (T, R, prefix rows, weights kept): in one launch, sharing key tiles
+    "shared_R16_P96": ("shared", 1120, (16, 96, False)), "shared_R64_P8192": ("shared", 100, (64, 8192, False)),
+    "weighted_R16_P96": ("shared", 1120, (16, 96, True)),
+    # 16 slots of T rows cut to B, in the 28 layers of the talker or in one
+    "evict_T1408_28": ("evict", 1408, (1024, 28)), "evict_T1408_1": ("evict", 1408, (1024, 1)),
     # calibration: what a chain of dependent kernels costs on this GPU without any attention work
     "calib_tiny": ("calib", 0, None), "calib_copy_4.6MB": ("calib", 4616192, None),
 }
@@ -187,6 +193,46 @@ def grouped_case(T, R, sets, dev):
     return fns, R * s.layer_bytes(T), "byte"
 
 
+def shared_case(T, x, sets, dev):
+    """R requests of T own rows behind P shared ones (sk_decode_attention_shared); work = the prefix once, every own
+    row once, the weights read and written."""
+    R, P, weights = x
+    s = W.C3
+    max_len = T + 32
+    g = torch.Generator(device=dev).manual_seed(0)
+    fns = []
+    for _ in range(sets):
+        K, V = (torch.randn(R, s.nkv, max_len, s.hd, device=dev, generator=g, dtype=torch.bfloat16) for _ in range(2))
+        Kp, Vp = (torch.randn(s.nkv, P, s.hd, device=dev, generator=g, dtype=torch.bfloat16) for _ in range(2))
+        mass = torch.zeros(R, s.nkv, max_len, device=dev) if weights else None
+        pos = torch.full((R,), P + T - 1, device=dev, dtype=torch.int64)
+        rope = qwen3.rope_table(P + max_len, s.theta, s.hd, dev)
+        qkv = torch.randn(R, (s.nq + 2 * s.nkv) * s.hd, device=dev, generator=g)
+        qn, out = torch.ones(s.hd, device=dev), torch.empty(R, s.nq * s.hd, device=dev)
+        plan = ops.shared_decode_plan(K, V, pos, rope, s.nq, s.eps, Kp=Kp, Vp=Vp, mass=mass)
+        fns.append(lambda plan=plan, qkv=qkv, qn=qn, out=out: ops.decode_attention_shared(plan, qkv, qn, qn, out=out))
+    work = (P + R * T) * s.nkv * s.hd * 4 + R * (2 * s.nq + 2 * s.nkv) * s.hd * 4 + (R * s.nkv * T * 8 if weights else 0)
+    return fns, work, "byte"
+
+
+def evict_case(T, x, sets, dev):
+    """16 slots of T rows cut to `keep` by mass (sk_cache_evict), over `layers` layers' caches; work = the masses and
+    the kept rows read and written."""
+    keep, layers = x
+    s = W.C3
+    R = 16
+    g = torch.Generator(device=dev).manual_seed(0)
+    fns = []
+    for _ in range(sets):
+        K, V = (torch.randn(layers, R, s.nkv, T, s.hd, device=dev, generator=g, dtype=torch.bfloat16) for _ in range(2))
+        mass = torch.rand(layers, R, s.nkv, T, device=dev, generator=g)
+        rows = torch.full((R,), T, device=dev, dtype=torch.int64)
+        out = tuple(torch.empty_like(t[..., :keep, :]) for t in (K, V)) + (torch.empty_like(mass[..., :keep]), rows.clone())
+        plan = ops.cache_evict_plan(K, V, mass, rows, keep, first=4, recent=64, out=out)
+        fns.append(lambda plan=plan: ops.cache_evict(plan))
+    return fns, layers * R * s.nkv * (T * 4 + keep * (s.hd * 8 + 4)), "byte"
+
+
 def linear_case(mnk, impl, sets, dev):
     """y = x·wᵀ (engine/fused.py:262-264) on sk_dit_linear or on torch's F.linear (cuBLAS); work = 2·M·N·K."""
     M, N, K = mnk
@@ -253,6 +299,10 @@ def main():
         fns, work, unit = block_case(x, B, a.sets, dev)
     elif kind == "grouped":
         fns, work, unit = grouped_case(x, B, a.sets, dev)
+    elif kind == "shared":
+        fns, work, unit = shared_case(x, B, a.sets, dev)
+    elif kind == "evict":
+        fns, work, unit = evict_case(x, B, a.sets, dev)
     else:
         fns, work, unit = calib_case(x, a.sets, dev)
     for f in fns:
@@ -310,6 +360,10 @@ def _shape(kind, x, B):
         if kind == "grouped":
             d["requests"] = B
         return d
+    if kind == "shared":
+        return {"T": x, "requests": B[0], "prefix": B[1], "weights": B[2], "nq": W.C3.nq, "nkv": W.C3.nkv, "hd": W.C3.hd}
+    if kind == "evict":
+        return {"T": x, "keep": B[0], "layers": B[1], "slots": 16, "nkv": W.C3.nkv, "hd": W.C3.hd}
     return {"bytes": x}
 
 

@@ -3,9 +3,9 @@ prefix, against a float64 restatement. The caches behind the rows in use, the pr
 and the masses of unused rows hold NaN throughout, so nothing may come from there.
 
 Bars (relative L2). fp32 activations out of fp32 caches: 1e-5, the package's parity bar. fp32 activations out
-of bf16 caches: q is split into two bf16 terms (each rounding at most 2^-8 of what it rounds: 2^-16 of q
-together) and so are the weights, rms errors 2^-16 / sqrt(3) = 8.8e-6 of a score of about 1 and of a weight,
-independent over the keys, so their average over the keys is below 1e-5 as well. bf16 activations: the result
+of bf16 caches: q and the weights are split into two bf16 terms at least (each rounding at most 2^-8 of what it
+rounds: 2^-16 of the number together, three leave 2^-24), rms errors 2^-16 / sqrt(3) = 8.8e-6 of a score of about 1
+and of a weight, independent over the keys, so their average over the keys is below 1e-5 as well. bf16 activations: the result
 (2^-8) and the weights (2^-8, averaged over keys) are each rounded once: 2^-7. Masses: a weight's error as
 above, 1e-5. Appended rows: one rounding to the cache dtype of a value computed in fp32 (bf16: one step, 2^-7
 of the element, where fp32 and float64 fall on two sides of a border, and 2e-6 where the rotation's two products,
@@ -187,6 +187,80 @@ TYPES = {"bf16 cache, f32 io": (BF, F32), "bf16 cache, bf16 io": (BF, BF), "f32 
 def test_step_against_float64(cuda, case, types, mass):
     cdt, io = TYPES[types]
     Step(cuda, cdt=cdt, io=io, mass=mass, seed=len(case), **CASES[case]).run()
+
+
+# Prefixes long enough that the requests share their tiles instead of reading them each (bf16 caches:
+# R * nkv * P rows of K and V past 12 MB + R * nkv / 3 MB), by query rows n of a key/value head.
+TILED = {
+    "n = 2": dict(lens=[150], P=4801, nq=16, nkv=8, hd=128),
+    "n = 8, the most of the short form": dict(lens=[40, 0, 129, 3], P=3900, nq=4, nkv=2, hd=128),
+    "n = 9, the least of the long form": dict(lens=[0, 1, 2, 3, 127, 128, 129, 255, 256], P=3500, nq=1, nkv=1, hd=128),
+    "n = 10, an idle slot among them": dict(lens=[40, -1, 0, 129, 3], P=3201, nq=4, nkv=2, hd=128),
+    "n = 96, groups of eight": dict(lens=[(29 * i) % 300 for i in range(12)], P=1801, nq=16, nkv=2, hd=128),
+    "n = 128": dict(lens=[(7 * i) % 60 for i in range(64)], P=1152, nq=4, nkv=2, hd=128),
+    "n = 140, two row tiles": dict(lens=[5 + 3 * (i % 7) for i in range(70)], P=899, nq=4, nkv=2, hd=128),
+    "n = 141, a group over a row tile's edge": dict(lens=[i for i in range(47)], P=1000, nq=6, nkv=2, hd=128),
+    "n = 300, three row tiles, groups of five": dict(lens=[(11 * i) % 200 for i in range(60)], P=1201, nq=5, nkv=1, hd=128),
+    "heads of 64, groups of five": dict(lens=[(41 * i) % 333 for i in range(24)], P=1701, nq=35, nkv=7, hd=64),
+    "heads of 64, n = 3": dict(lens=[17, 500, 0], P=18001, nq=1, nkv=1, hd=64),
+    "strided caches": dict(lens=[40, 0, 129, 3, 9], P=3301, nq=6, nkv=3, hd=128, strided=8),
+    "evicted before": dict(lens=[500, 131, 7], P=2801, nq=16, nkv=8, hd=128, gone=4000),
+    "all idle": dict(lens=[-1, -1], P=4001, nq=16, nkv=8, hd=128),
+}
+
+
+@pytest.mark.parametrize("mass", [False, True])
+@pytest.mark.parametrize("io", [F32, BF])
+@pytest.mark.parametrize("case", TILED)
+def test_shared_tiles_against_float64(cuda, case, io, mass):
+    a = TILED[case]
+    heads = len(a["lens"]) * a["nkv"]
+    assert heads * a["P"] * 4 * a["hd"] > (12 << 20) + heads * (1 << 20) // 3
+    Step(cuda, io=io, mass=mass, seed=len(case), **a).run()
+
+
+@pytest.mark.parametrize("mass", [False, True])
+@pytest.mark.parametrize("R,P,nq,nkv,hd", [(1024, 2100, 2, 1, 64), (300, 900, 4, 4, 128), (100, 10601, 3, 1, 128)])
+def test_shared_tiles_of_fp32_caches_against_float64(cuda, R, P, nq, nkv, hd, mass):
+    """More than 1 GB of rows if every request read the prefix for itself."""
+    assert R * nkv * P * 8 * hd > 1 << 30
+    lens = [-1 if i % 19 == 5 else (7 * i) % 67 for i in range(R)]
+    Step(cuda, lens, P, nq, nkv, hd, cdt=F32, mass=mass, seed=R).run()
+
+
+@pytest.mark.parametrize("io", [F32, BF])
+def test_shared_tiles_captured_twice_with_one_workspace(cuda, io):
+    """Two captured steps and an eager one, all of one plan's workspace, in turn on one stream."""
+    s = Step(cuda, [(31 * i) % 400 for i in range(12)], 1500, 16, 8, 128, io=io, mass=True, seed=24)
+    want, before, m0, plan = s.want(), s.before(), s.mass.clone(), s.plan()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            ops.decode_attention_shared(plan, s.qkv, s.qn, s.kn, out=s.out)
+        graphs.append(g)
+    run = [graphs[0].replay, graphs[1].replay, lambda: ops.decode_attention_shared(plan, s.qkv, s.qn, s.kn, out=s.out)]
+    for i in range(9):
+        s.out.fill_(7.0)
+        s.mass.copy_(m0)
+        run[i % 3]()
+    s.check(want, before)
+
+
+def test_shared_tiles_on_two_streams(cuda):
+    steps = [Step(cuda, [(31 * i) % 300 for i in range(12)], 1500, 16, 8, 128, mass=True, seed=s) for s in (26, 27)]
+    want, before = [s.want() for s in steps], [s.before() for s in steps]
+    plans, m0 = [s.plan() for s in steps], [s.mass.clone() for s in steps]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in steps]
+    for _ in range(20):
+        for s, p, st, m in zip(steps, plans, streams, m0):
+            with torch.cuda.stream(st):
+                s.mass.copy_(m)
+                ops.decode_attention_shared(p, s.qkv, s.qn, s.kn, out=s.out)
+    torch.cuda.synchronize()
+    for s, w, b in zip(steps, want, before):
+        s.check(w, b)
 
 
 @pytest.mark.parametrize("cdt", [BF, F32])
