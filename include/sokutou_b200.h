@@ -396,8 +396,8 @@ SK_API size_t sk_decode_shared_workspace_bytes(const SkSharedDecode* d);
 
 /*
  * One decode step of one layer for R requests whose caches all continue the same prefix (one voice
- * prompt, one system prompt): the prefix's keys and values are read once for all requests together, each
- * request's own rows once. No counterpart in the reference, which serves one request at a time
+ * prompt, one system prompt): the prefix's keys and values are read once for all requests together (a short
+ * prefix by each request, out of L2), each request's own rows once. No counterpart in the reference, which serves one request at a time
  * (README.md:186); per request the arithmetic of its `attn` kernel (qwen3/kernels.py:338-414).
  *
  * For every request r with pos[r] >= 0, n = rows[r] (or pos[r] - P) own rows and group g = nq / nkv:
@@ -413,7 +413,7 @@ SK_API size_t sk_decode_shared_workspace_bytes(const SkSharedDecode* d);
  *
  *   qkv      : [R][(nq + 2*nkv) * hd] = [q heads | k heads | v heads], qkv_stride between rows
  *   qn, kn   : fp32 [hd]
- *   out      : [R][nq * hd], out_stride between rows
+ *   out      : [R][nq * hd], out_stride between rows; shares no element with qkv (else SK_ERR_INVALID_ARG)
  *   Sums, softmax statistics and the accumulated output are fp32. bf16 caches run on the tensor cores
  *   with q as a sum of two bf16 terms (2^-16 of it at most is left out) and the weights in one or two; with an
  *   fp32 `out` both in three (2^-24), or in two where more than 8 query heads share a key tile of the prefix.

@@ -465,6 +465,17 @@ static bool use_direct(const Params& p, int row_bytes) {
   return heads * p.P * 2 * row_bytes <= (p.f32 ? 1024 * mb : 12 * mb + heads * mb / 3);
 }
 
+// Whether rows [R] of `na` bytes at `a` and of `nb` bytes at `b` share a byte, the strides in bytes. Rows of two
+// strides that lie between one another count as if they did.
+static bool rows_meet(const void* a, long long na, long long stride_a, const void* b, long long nb, long long stride_b, int R) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  if (R == 1) stride_a = stride_b = 0;
+  if (x + (R - 1) * stride_a + na <= y || y + (R - 1) * stride_b + nb <= x) return false;
+  if (R == 1 || stride_a != stride_b) return true;
+  const uintptr_t d = y >= x ? (y - x) % stride_a : (stride_a - (x - y) % stride_a) % stride_a;  // b's place in a row of a's
+  return (long long)d < na || (long long)d + nb > stride_a;
+}
+
 static WsLayout layout_of(const SkSharedDecode* d) {
   return d->cache_dtype == SK_BF16
              ? ws_layout<CutTc>(d->R, d->nq, d->nkv, d->hd, d->prefix_len, d->max_len, d->mass != nullptr)
@@ -505,6 +516,9 @@ extern "C" int sk_decode_attention_shared(const SkSharedDecode* d, const void* q
   }
   if (d->R > 1 && (d->qkv_stride < (long long)(d->nq + 2 * d->nkv) * hd || d->qkv_stride % (q16 ? 8 : 4) ||
                    d->out_stride < (long long)d->nq * hd || d->out_stride % (o16 ? 8 : 4)))
+    return SK_ERR_INVALID_ARG;
+  if (rows_meet(qkv, (long long)(d->nq + 2 * d->nkv) * hd * (q16 ? 2 : 4), d->qkv_stride * (q16 ? 2 : 4), out,
+                (long long)d->nq * hd * (o16 ? 2 : 4), d->out_stride * (o16 ? 2 : 4), d->R))
     return SK_ERR_INVALID_ARG;
   if (d->mass && ((reinterpret_cast<uintptr_t>(d->mass) & 3) || (d->R > 1 && d->mass_request_stride < 1) ||
                   (d->nkv > 1 && d->mass_head_stride < 1)))

@@ -534,7 +534,7 @@ def decode_attention_shared(plan: SharedDecodePlan, qkv: torch.Tensor, qn: torch
     """One decode step of one layer for all requests of `plan`: appends each live request's k and v to its own
     cache (row rows[r]), attends over the shared prefix and its own rows, adds the own rows' attention
     weights to the plan's mass. qkv (R, (nq + 2*nkv)*hd); qn, kn float32 (hd,); returns out (R, nq*hd), rows
-    of idle slots left as they were. The prefix is read once for all requests."""
+    of idle slots left as they were (not set in an out made here); out may not share elements with qkv."""
     if out is None:
         _need(plan.out_stride[0] == plan.out_shape[1], "a plan with an out_stride needs out=")
         out = torch.empty(plan.out_shape, device=plan.device, dtype=plan.out_dtype)

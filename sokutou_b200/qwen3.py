@@ -91,11 +91,15 @@ class TalkerGroup:
                                               mass=None if self.mass is None else self.mass[i], qkv_dtype=act_dtype,
                                               out_dtype=act_dtype, workspace=ws) for i in range(n_layers)]
         self._evict_plans: dict[tuple[int, int, int], ops.CacheEvictPlan] = {}
+        self._evict_ws = None  # of all budgets: a step evicts by one
 
     def start(self, slot: int, rows: int = 0) -> None:
-        """A request takes the slot, `rows` own rows of its caches already filled (by a prefill, or a copy)."""
+        """A request takes the slot, `rows` own rows of its caches already filled (by a prefill, or a copy); their
+        weights count from zero."""
         if not 0 <= slot < self.R or not 0 <= rows < self.max_len:
             raise ValueError(f"slot {slot} of {self.R}, {rows} rows of {self.max_len}")
+        if rows and self.mass is not None:
+            self.mass[:, slot, :, :rows] = 0
         self.pos[slot], self.rows[slot], self._live[slot] = self.prefix_len + rows, rows, 1
 
     def stop(self, slot: int) -> None:
@@ -119,5 +123,8 @@ class TalkerGroup:
             raise ValueError("evict needs track_mass=True")
         key = (keep, first, recent)
         if key not in self._evict_plans:
-            self._evict_plans[key] = ops.cache_evict_plan(self.k, self.v, self.mass, self.rows, keep, first, recent)
+            args = (self.k, self.v, self.mass, self.rows)
+            if self._evict_ws is None:
+                self._evict_ws = ops.cache_evict_plan(*args, self.max_len).workspace
+            self._evict_plans[key] = ops.cache_evict_plan(*args, keep, first, recent, workspace=self._evict_ws)
         ops.cache_evict(self._evict_plans[key])

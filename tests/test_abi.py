@@ -97,6 +97,13 @@ def test_shared_decode_refusals_without_device(native_lib):
                dict(mass=8, mass_request_stride=0, mass_head_stride=64), dict(mass=6)):
         assert call(**kw) == -1, kw
     assert call(workspace=None) == -5 and call(workspace=(8 << 20) + 16) == -5 and call(ws_bytes=size() - 1) == -5
+    # out over qkv, one row of it, one element of it; then side by side in rows of 48 * 128, which only a device is missing for
+    at, wide = 1 << 22, dict(qkv_stride=48 * 128, out_stride=48 * 128)
+    for kw in (dict(out=at), dict(out=at + 3 * 32 * 128 * 4), dict(out=at - 4 * 16 * 128 * 4 + 16), dict(out=at, R=1),
+               dict(out=at + 32 * 128 * 4 - 16, **wide), dict(out=at - 16 * 128 * 4 + 16, **wide)):
+        assert call(qkv=at, **kw) == -1, kw
+    for kw in (dict(out=at + 32 * 128 * 4, **wide), dict(out=at - 16 * 128 * 4, **wide), dict(out=at + 4 * 32 * 128 * 4)):
+        assert call(qkv=at, ws_bytes=0, **kw) == -5, kw
     assert size() > 0 and size(mass=256) > size() > size(prefix_len=0) and size(R=5) > size()
 
 

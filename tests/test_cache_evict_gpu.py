@@ -291,3 +291,31 @@ def test_bounded_streams_against_float64(cuda, cdt):
                 for t in (ks, vs, ms):
                     t[:] = [t[j] for j in at]
     assert ops.device_error() == 0
+
+
+def test_group_slots_taken_again_and_budgets_changed(cuda):
+    """A slot's next request does not inherit the weights of the last one, and budgets share one workspace."""
+    from sokutou_b200.qwen3 import TalkerGroup
+
+    tg = TalkerGroup(2, 3, 4, 2, 64, 1e6, 1e-6, cuda, track_mass=True)
+    tg.mass.fill_(5.0)
+    tg.start(1, rows=40)
+    assert (tg.mass[:, 1, :, :40] == 0).all() and (tg.mass[:, 0] == 5).all() and (tg.mass[:, 1, :, 40:] == 5).all()
+    tg.mass.copy_(torch.rand(tg.mass.shape, device=cuda))
+    for keep in (30, 20, 10):
+        before, k = tg.mass.clone(), tg.k.normal_().clone()
+        n = int(tg.rows[1])
+        tg.evict(keep, 2, 3)
+        assert tg.rows.tolist() == [0, keep, 0] and tg.pos.tolist() == [-1, 40, -1]
+        for i in range(2):
+            for h in range(2):
+                at = kept_rows(before[i, 1, h].cpu().numpy(), n, keep, 2, 3)
+                assert torch.equal(tg.mass[i, 1, h, :keep], before[i, 1, h][at])
+                assert torch.equal(tg.k[i, 1, h, :keep], k[i, 1, h][at])
+    assert len({p.workspace.data_ptr() for p in tg._evict_plans.values()}) == 1 and ops.device_error() == 0
+    with pytest.raises(ValueError):
+        tg.start(3)
+    with pytest.raises(ValueError):
+        tg.start(0, rows=64)
+    with pytest.raises(ValueError):
+        TalkerGroup(1, 1, 4, 2, 64, 1e6, 1e-6, cuda).evict(10)
