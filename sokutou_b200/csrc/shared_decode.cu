@@ -541,6 +541,7 @@ extern "C" int sk_decode_attention_shared(const SkSharedDecode* d, const void* q
   p.R = d->R, p.nq = d->nq, p.nkv = d->nkv, p.g = d->nq / d->nkv;
   p.P = d->prefix_len, p.max_len = d->max_len, p.rope_len = d->rope_len;
   p.f32 = d->cache_dtype == SK_F32, p.qkv_bf16 = q16, p.out_bf16 = o16;
+  p.long_sums = !p.f32 && !o16 && long_sums_of<CutTc>(d->R, d->nq, d->nkv, d->prefix_len, d->max_len);
   p.eps = d->eps;
   p.q_scale = (d->scale > 0.f ? d->scale : (hd == 128 ? 0.08838834764831845f : 0.125f)) * kLog2e;
   uint8_t* ws = reinterpret_cast<uint8_t*>(d->workspace);

@@ -5,13 +5,15 @@
 // query rows) an item of ceil(P / KT) tiles — query row i = r*g + h of a head, all requests together —, then
 // the own rows, per (request, key/value head) an item of ceil(n / KT) tiles. All tiles lie in one row, item
 // after item, each at its cost from the start (see Tiles), and the row is cut into equal shares for the CTAs
-// of the grid, a tile falling to the share that its start lies in: every CTA has the same to do whatever
-// the lengths are, and an item is cut only where a share ends. The part of an item that one CTA does is a
-// segment; it leaves one partial (running max, sum, unnormalised output) per query row. Along the row the
-// pair (CTA, item) never steps back in either and moves in one at least, so CTA + item numbers a segment's
-// place in the workspace uniquely. The lengths are read on the device, so one captured graph serves every
+// of the grid, as many to each, one unless that would be long (see kShare), a tile falling to the share that its
+// start lies in: every CTA has the same to do whatever the lengths are, and an item is cut only where a share
+// ends. The part of an item in one share is a segment; it leaves one partial (running max, sum, unnormalised
+// output) per query row. Along the row the pair (share, item) never steps back in either and moves in one at
+// least, so share + item numbers a segment's place in the workspace uniquely. The lengths are read on the device, so one captured graph serves every
 // step.
 #pragma once
+
+#include <algorithm>
 
 #include "sk_common.cuh"
 
@@ -62,6 +64,7 @@ struct Params {
   long long qkv_stride, out_stride;
   int R, nq, nkv, g, P, max_len, rope_len;
   int f32, qkv_bf16, out_bf16;  // types of the caches, qkv and out
+  int long_sums;       // shares of at most kShare, several to a CTA
   float eps, q_scale;  // softmax scale * log2(e): scores come out in the log2 domain
   float* po;           // prefix partials [CTA + item][RT][hd]; ml [..][RT][2]
   float* pml;
@@ -90,13 +93,40 @@ __host__ inline bool too_many_tiles(long long R, long long g, long long nkv, lon
 
 __host__ __device__ inline long long align_up(long long x, long long a) { return (x + a - 1) / a * a; }
 
+// The sums that tensor memory holds are cut off, not rounded, at every addition, which takes 1.2e-7 of a sum away per
+// tile of its segment, or 2.2e-7 with the weights in two products (measured). Where fp32 goes out and segments could
+// pass kLongFew or kLongMany tiles (see long_sums_of), a CTA takes several shares that cost at most kShare each, 40
+// tiles of few query rows or 20 of many. Relative L2 of the output, one share for each CTA and so: one request behind
+// 300001 rows 2.0e-5 and 4.9e-6 (187 and 199 us), eight behind 200001 rows 3.1e-5 and 8.6e-6 (221 and 252 us), two
+// with 150001 rows of their own 2.1e-5 and 5.6e-6 (184 and 317 us). Not otherwise: the walk over shares is code that
+// other calls need not fetch (64 requests behind 8192 rows 62 us with it, 55.6 without).
+constexpr int kShare = 80, kLongFew = 48, kLongMany = 26, kFewRows = 8;
+template <class Cut>
+__host__ inline long long prefix_cost(long long rows, long long tiles) {  // of an item, as in tiles_of
+  return rows > kFewRows ? (rows > 64 ? 8 : 4) + 4 * tiles : 2 + 2 * tiles;
+}
+
+template <class Cut>
+__host__ inline bool long_sums_of(int R, int nq, int nkv, int P, int max_len) {
+  const long long g = nq / nkv, rows = R * g, tp = (P + Cut::KT - 1) / Cut::KT, to = (max_len + Cut::KT - 1) / Cut::KT;
+  const long long items = P > 0 ? nkv * ((rows + Cut::RT - 1) / Cut::RT) : 0;
+  const long long share = (items * prefix_cost<Cut>(rows, tp) + (long long)R * nkv * (2 + 2 * to)) / Cut::G + 1;
+  return std::min(share / 2, to) > kLongFew ||
+         (rows > kFewRows ? std::min(share / 4, tp) > kLongMany : std::min(share / 2, tp) > kLongFew);
+}
+
 struct WsLayout {
   long long po, pml, oo, oml, sc, sc_stride, bytes, slots_p, slots_o;
 };
 template <class Cut>
 __host__ inline WsLayout ws_layout(int R, int nq, int nkv, int hd, int P, int max_len, bool mass) {
   const long long g = nq / nkv, items_p = P > 0 ? (long long)nkv * ((R * g + Cut::RT - 1) / Cut::RT) : 0;
-  const long long slots_p = P > 0 ? items_p + Cut::G : 0, slots_o = (long long)R * nkv + Cut::G;
+  const long long tp = (P + Cut::KT - 1) / Cut::KT, to = (max_len + Cut::KT - 1) / Cut::KT;
+  const long long cost_p = items_p * prefix_cost<Cut>(R * g, tp), cost = cost_p + (long long)R * nkv * (2 + 2 * to);
+  const long long shares = Cut::G * (Cut::kWeighted ? cost / (Cut::G * kShare) + 1 : 1);
+  // the prefix's shares: Cut::G at the most while a CTA has one, later each costs kShare / 2 at least
+  const long long shares_p = std::max((long long)Cut::G, std::min(shares, cost_p / (kShare / 2) + 2));
+  const long long slots_p = P > 0 ? items_p + shares_p : 0, slots_o = (long long)R * nkv + shares;
   WsLayout w;
   w.slots_p = slots_p, w.slots_o = slots_o;
   long long at = 0;
@@ -135,14 +165,13 @@ __device__ __forceinline__ int own_rows(const Params& p, int r, bool* bad, int* 
 // take the tensor cores and the exponentials for about twice as long, and their rows are many). With every
 // tile at 1 the prefix's CTAs took 133 thousand cycles when the others took 75, at 64 requests behind 8192 rows
 // (74 us, 54.7 so; 60.7 with 4 in the place of 8, 59.0 with 12). With fewer tiles each costs 1 and is a CTA's own.
-constexpr int kFewRows = 8;
-
 struct Tiles {
   int tp, nrt;         // tiles of a prefix item; prefix items per head
   int items_p;         // prefix items
   int shift_p, first_p, shift_o, first_o;
   int prefix;          // cost of all prefix items
-  int each, more;      // a share costs `each`, one more for the first `more` CTAs
+  int per;             // shares of a CTA: 1 unless p.long_sums
+  int each, more;      // a share costs `each`, one more for the first `more` shares
   __device__ __forceinline__ int cost_p() const { return first_p + (tp << shift_p); }
 };
 // own_tiles, own_items: of all requests, per head.
@@ -163,12 +192,13 @@ __device__ __forceinline__ Tiles tiles_of(const Params& p, int own_tiles, int ow
     total = t.items_p * t.tp + p.nkv * own_tiles;
   }
   t.prefix = t.items_p * t.cost_p();
-  t.each = (int)((uint32_t)total / Cut::G);
-  t.more = total - t.each * Cut::G;
+  t.per = p.long_sums ? (int)((uint32_t)total / (Cut::G * kShare)) + 1 : 1;
+  t.each = (int)((uint32_t)total / (Cut::G * t.per));
+  t.more = total - t.each * Cut::G * t.per;
   return t;
 }
 __device__ __forceinline__ int share_begin(const Tiles& t, int c) { return c * t.each + min(c, t.more); }
-__device__ __forceinline__ int share_of(const Tiles& t, int at) {  // the CTA whose share holds cost position `at`
+__device__ __forceinline__ int share_of(const Tiles& t, int at) {  // the share that holds cost position `at`
   const uint32_t cut = (uint32_t)t.more * (t.each + 1);
   return (int)((uint32_t)at < cut ? (uint32_t)at / (t.each + 1) : t.more + ((uint32_t)at - cut) / t.each);
 }
@@ -227,7 +257,7 @@ __device__ __forceinline__ Tiles scan_tiles(const Params& p, const Lens& s, bool
   return t;
 }
 
-// The segments of a CTA's share, one after another.
+// The segments of a CTA's shares, one after another.
 struct Segments {
   bool prefix;
   int item;     // prefix: kvh * nrt + rt; own: r * nkv + kvh
@@ -235,12 +265,14 @@ struct Segments {
   int t0, t1;   // tiles of the item
   int n_keys;   // rows of the item (prefix: P; own: n)
   int at, end;  // cost positions of the item's start and of the share's end
+  int share;    // this segment's share
 
-  // The first segment of CTA c's share; false: the share is empty.
-  template <int KT>
+  // The first segment of CTA c = blockIdx.x; false: it has none.
+  template <int KT, bool LONG = false>
   __device__ __forceinline__ bool first(const Params& p, const Tiles& t, const Lens& s, int c) {
-    const int from = share_begin(t, c);
-    end = share_begin(t, c + 1);
+    share = LONG ? c * t.per : c;
+    const int from = share_begin(t, share);
+    end = share_begin(t, share + 1);
     if (from >= end) return false;
     int off, tiles, shift, extra;
     if (from < t.prefix) {
@@ -274,15 +306,27 @@ struct Segments {
     off = from - at;
     // the first tile that starts at `off` or later; past the item's last: the next item's first
     t0 = off == 0 ? 0 : max(1, (off - extra + (1 << shift) - 1) >> shift);
-    if (t0 >= tiles) return next<KT>(p, t, s);
+    if (t0 >= tiles) {
+      t1 = tiles;
+      return next<KT, LONG>(p, t, s);
+    }
     take(tiles, extra, shift);
     return true;
   }
   // Steps on; false after the last. Items follow one another without gaps, so no division is needed.
-  template <int KT>
+  template <int KT, bool LONG = false>
   __device__ __forceinline__ bool next(const Params& p, const Tiles& t, const Lens& s) {
-    at += prefix ? t.cost_p() : s.cum[r + 1] - s.cum[r];
-    if (at >= end) return false;
+    const bool rest = LONG && t1 < (prefix ? t.tp : (n_keys + KT - 1) / KT);  // the share ended within the item
+    if (!rest) at += prefix ? t.cost_p() : s.cum[r + 1] - s.cum[r];
+    if (rest || at >= end) {
+      if (!LONG || ++share == (int)(blockIdx.x + 1) * t.per) return false;
+      end = share_begin(t, share + 1);
+    }
+    if (rest) {
+      t0 = t1;
+      take(prefix ? t.tp : (n_keys + KT - 1) / KT, prefix ? t.first_p : t.first_o, prefix ? t.shift_p : t.shift_o);
+      return true;
+    }
     t0 = 0;
     if (prefix) {
       if (++r == t.nrt) {

@@ -24,7 +24,8 @@
 // more product per tile, which runs while memory is waited for; with a single term a score of 10 is off by 0.02.
 // The weights P are rounded to bf16 where the output is (2^-8 either way); P_SPLIT (fp32 outputs) takes them in two
 // terms as well, and with n <= 8, where they are columns that are there anyway, q and P in three (2^-24, as fp32).
-// With n > 8 neither shared nor tensor memory has room for a third: 4e-6 of the output, measured, against 5e-7.
+// With n > 8 neither shared nor tensor memory has room for a third: 4e-6 of the output, measured, against 5e-7 (both
+// more behind long prefixes: see kShare).
 // The running sum is of the unrounded weights, in fp32.
 #include <type_traits>
 
@@ -184,7 +185,7 @@ __device__ __forceinline__ int rows_of(const Params& p, const Segments& s) {
 // so that one's rows can be written while the other's are read (the rest of a product is ignored).
 __device__ __forceinline__ int base_of(int n, int seg) { return n <= 64 ? 64 * (seg & 1) : 0; }
 
-template <int HD, bool P_SPLIT>
+template <int HD, bool P_SPLIT, bool LONG>
 __global__ void __maxnreg__(kLaunchRegs)
     tiles_tc_kernel(const __grid_constant__ CUtensorMap tmKp, const __grid_constant__ CUtensorMap tmVp,
                     const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -242,7 +243,7 @@ __global__ void __maxnreg__(kLaunchRegs)
     const Tiles tl = scan_tiles<CutTc>(p, ls, c == 0);
     if (lane == 0) {
       Segments sg;
-      misc[1] = sg.first<CutTc::KT>(p, tl, ls, c);
+      misc[1] = sg.first<CutTc::KT, LONG>(p, tl, ls, c);
       *reinterpret_cast<Tiles*>(smem + S::OFF_TILES) = tl;
       *reinterpret_cast<Segments*>(smem + S::OFF_SEG) = sg;
     }
@@ -333,7 +334,7 @@ __global__ void __maxnreg__(kLaunchRegs)
       // ---------------------------------------------------------------- TMA producer
       int i = 0;
       bool ok = true;
-      for (; more && ok; more = sg.next<CutTc::KT>(p, tl, ls)) {
+      for (; more && ok; more = sg.next<CutTc::KT, LONG>(p, tl, ls)) {
         const MapOrder& o = args.order;
         for (int t = sg.t0; t < sg.t1 && ok; ++t, ++i) {
           // K, then V of the tile (one copy of the code: what(0), what(1))
@@ -371,7 +372,7 @@ __global__ void __maxnreg__(kLaunchRegs)
       const uint64_t k0 = smem_desc_sw128(sbase + S::OFF_K, 16, 1024);
       int i = 0, seg = 0;
       bool ok = true;
-      for (; more && ok; more = sg.next<CutTc::KT>(p, tl, ls), ++seg) {
+      for (; more && ok; more = sg.next<CutTc::KT, LONG>(p, tl, ls), ++seg) {
         const bool few = rows_of(p, sg) <= kFew;
         if (!(ok = wait_on(&q_full[seg & 1], seg >> 1, p.err))) break;
         for (int t = sg.t0; t < sg.t1; ++t, ++i) {
@@ -407,7 +408,7 @@ __global__ void __maxnreg__(kLaunchRegs)
       const uint64_t v0 = smem_desc_sw128(sbase + S::OFF_V, 16384, 1024), p0 = smem_desc_sw128(sbase + S::OFF_PT, 16, 1024);
       int i = 0, seg = 0;
       bool ok = true;
-      for (; more && ok; more = sg.next<CutTc::KT>(p, tl, ls), ++seg) {
+      for (; more && ok; more = sg.next<CutTc::KT, LONG>(p, tl, ls), ++seg) {
         const bool few = rows_of(p, sg) <= kFew;
         const uint32_t oc = tO + (seg & 1) * 128;
         if (seg >= 2 && !(ok = wait_on(&o_free[seg & 1], (seg - 2) >> 1, p.err))) break;
@@ -461,7 +462,7 @@ __global__ void __maxnreg__(kLaunchRegs)
         wait(&so_full[seg & 1], seg >> 1);
         wait(&ml_full[seg & 1], seg >> 1);
         tc_fence_after();
-        long long slot = (long long)c + sg.item;
+        long long slot = (long long)(LONG ? sg.share : c) + sg.item;
         if (!SK_INB(slot < (sg.prefix ? p.slots_p : p.slots_o), p.err)) slot = 0;
         const long long row0 = sg.prefix ? slot * CutTc::RT : slot * p.g;  // first partial row
         float* o = (sg.prefix ? p.po : p.oo) + row0 * HD;
@@ -503,7 +504,7 @@ __global__ void __maxnreg__(kLaunchRegs)
         sg = nx;
         more = another;
       }
-      if (another) another = nx.next<CutTc::KT>(p, tl, ls);
+      if (another) another = nx.next<CutTc::KT, LONG>(p, tl, ls);
     }
     if (warp < kWarpQo) {
       // ---------------------------------------------------------------- softmax
@@ -704,7 +705,7 @@ __global__ void __maxnreg__(kLaunchRegs)
         else
           *reinterpret_cast<float2*>(st + 2 * j) = make_float2(m_run, l_run);
       };
-      for (; more; more = sg.next<CutTc::KT>(p, tl, ls), ++seg) {
+      for (; more; more = sg.next<CutTc::KT, LONG>(p, tl, ls), ++seg) {
         const int n = rows_of(p, sg);
         if (n > kFew) {
           by_rows(n);
@@ -769,7 +770,7 @@ static bool prefix_map(CUtensorMap* m, const void* base, const Params& p, int hd
   return sk_make_map_bf16(m, base, 3, dims, str, box);
 }
 
-template <int HD, bool P_SPLIT>
+template <int HD, bool P_SPLIT, bool LONG = false>
 static int launch(const Params& p, cudaStream_t st) {
   CUtensorMap kp, vp, k, v;
   TcArgs a;
@@ -782,7 +783,7 @@ static int launch(const Params& p, cudaStream_t st) {
     vp = v;
   }
   const int smem = SmemTc<HD, P_SPLIT>::bytes(p.R);
-  if (cudaFuncSetAttribute(tiles_tc_kernel<HD, P_SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
+  if (cudaFuncSetAttribute(tiles_tc_kernel<HD, P_SPLIT, LONG>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
       cudaSuccess)
     return SK_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
@@ -795,10 +796,11 @@ static int launch(const Params& p, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, tiles_tc_kernel<HD, P_SPLIT>, kp, vp, k, v, a) == cudaSuccess ? SK_OK : SK_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, tiles_tc_kernel<HD, P_SPLIT, LONG>, kp, vp, k, v, a) == cudaSuccess ? SK_OK : SK_ERR_CUDA;
 }
 
 int launch_tiles_tc(const Params& p, int hd, bool p_split, cudaStream_t st) {
+  if (p.long_sums) return hd == 128 ? launch<128, true, true>(p, st) : launch<64, true, true>(p, st);
   if (hd == 128) return p_split ? launch<128, true>(p, st) : launch<128, false>(p, st);
   return p_split ? launch<64, true>(p, st) : launch<64, false>(p, st);
 }

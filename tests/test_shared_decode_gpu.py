@@ -228,6 +228,39 @@ def test_shared_tiles_of_fp32_caches_against_float64(cuda, R, P, nq, nkv, hd, ma
     Step(cuda, lens, P, nq, nkv, hd, cdt=F32, mass=mass, seed=R).run()
 
 
+@pytest.mark.parametrize("R,P,nq,nkv,hd,own", [(1, 300001, 16, 8, 128, 40), (8, 200001, 16, 8, 128, 3), (2, 500001, 3, 3, 64, 0),
+                                               (2, 100, 8, 8, 128, 150001)])
+def test_long_sums_stay_within_the_bar(cuda, R, P, nq, nkv, hd, own):
+    """Hundreds of tiles for every CTA: sums over them in tensor memory, whose additions cut off what does not fit,
+    have to be short (a tile of 128 keys takes 8 additions of 2^-24 of the sum per term and product, so the 40 tiles of
+    a partial take 40 * 8 * 2^-25 on the average, 9.5e-6, if every one of them cuts off half of a last place). The float64
+    restatement runs on the GPU."""
+    s = Step(cuda, [1] * R, 2, nq, nkv, hd, seed=30)  # small tensors of the right kinds, then the long ones
+    g = torch.Generator(device=cuda).manual_seed(31)
+    M = own + 8
+    s.K, s.V = (torch.randn(R, nkv, M, hd, device=cuda, generator=g, dtype=F32).to(BF) for _ in range(2))
+    s.Kp, s.Vp = (torch.randn(nkv, P, hd, device=cuda, generator=g, dtype=F32).to(BF) for _ in range(2))
+    s.rope = rope_table(P + M, hd).to(cuda)
+    s.rows.fill_(own)
+    s.pos.fill_(P + own)
+    ops.decode_attention_shared(s.plan(), s.qkv, s.qn, s.kn, out=s.out)
+    assert ops.device_error() == 0
+    d = lambda t: t.double()  # noqa: E731
+    c, sn = d(s.rope[P + own]).chunk(2)
+    for r in range(R):
+        x = d(s.qkv[r]).view(-1, hd)[:nq]
+        x = x * torch.rsqrt((x * x).mean(-1, keepdim=True) + EPS) * d(s.qn)
+        a, b = x.chunk(2, -1)
+        q = torch.cat([a * c - b * sn, b * c + a * sn], -1)
+        for h in range(nkv):
+            K = torch.cat([d(s.Kp[h]), d(s.K[r, h, :own + 1])])  # (the row appended as the cache holds it)
+            V = torch.cat([d(s.Vp[h]), d(s.V[r, h, :own + 1])])
+            for i in range(h * nq // nkv, (h + 1) * nq // nkv):
+                ref = torch.softmax(K @ q[i] * hd ** -0.5, 0) @ V
+                got = d(s.out[r, i * hd:(i + 1) * hd])
+                assert ((got - ref).norm() / ref.norm()).item() <= 1e-5, (r, i)
+
+
 @pytest.mark.parametrize("io", [F32, BF])
 def test_shared_tiles_captured_twice_with_one_workspace(cuda, io):
     """Two captured steps and an eager one, all of one plan's workspace, in turn on one stream."""
