@@ -460,7 +460,12 @@ static int launch_tc(const Params& p, bool p_split, cudaStream_t st) {
 // behind 1024 (67 MB); at one request 8.6 against 10.9 us behind 2048 rows and 18.4 against 13.6 behind 8192
 // (34 MB); at 64 requests 28 / 38 / 65 against 34 / 54 / 81 behind 512 (134 MB). fp32 caches have no tensor cores
 // to share rows on: 61 against 74 us for 16 requests behind 4096 rows (537 MB).
+// Caches that can hold long rows: a cluster has 8 CTAs at the most, the tiles' shares are even. 1 request behind 96
+// rows, own rows 1000 / 4000 / 8000 / 16000: 9.2 / 14.3 / 20.1 / 33.0 us against 12.1 / 15.3 / 16.3 / 18.7; 16 requests
+// 18.1 / 53.2 / 96.6 / 184 against 22.1 / 57.6 / 91.4 / 163. The host knows what a cache can hold, not what it does.
+constexpr int kLongCache = 8192;
 static bool use_direct(const Params& p, int row_bytes) {
+  if (!p.f32 && p.max_len > kLongCache) return false;
   const long long heads = (long long)p.R * p.nkv, mb = 1 << 20;
   return heads * p.P * 2 * row_bytes <= (p.f32 ? 1024 * mb : 12 * mb + heads * mb / 3);
 }

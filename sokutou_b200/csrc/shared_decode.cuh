@@ -98,7 +98,7 @@ __host__ __device__ inline long long align_up(long long x, long long a) { return
 // pass kLongFew or kLongMany tiles (see long_sums_of), a CTA takes several shares that cost at most kShare each, 40
 // tiles of few query rows or 20 of many. Relative L2 of the output, one share for each CTA and so: one request behind
 // 300001 rows 2.0e-5 and 4.9e-6 (187 and 199 us), eight behind 200001 rows 3.1e-5 and 8.6e-6 (221 and 252 us), two
-// with 150001 rows of their own 2.1e-5 and 5.6e-6 (184 and 317 us). Not otherwise: the walk over shares is code that
+// with 150001 rows of their own 2.1e-5 and 4.9e-6 (184 and 193 us). Not otherwise: the walk over shares is code that
 // other calls need not fetch (64 requests behind 8192 rows 62 us with it, 55.6 without).
 constexpr int kShare = 80, kLongFew = 48, kLongMany = 26, kFewRows = 8;
 template <class Cut>

@@ -229,7 +229,7 @@ def test_shared_tiles_of_fp32_caches_against_float64(cuda, R, P, nq, nkv, hd, ma
 
 
 @pytest.mark.parametrize("R,P,nq,nkv,hd,own", [(1, 300001, 16, 8, 128, 40), (8, 200001, 16, 8, 128, 3), (2, 500001, 3, 3, 64, 0),
-                                               (2, 100, 8, 8, 128, 150001)])
+                                               (2, 100, 8, 8, 128, 150001), (1, 96, 16, 8, 128, 8183), (1, 96, 16, 8, 128, 8185)])
 def test_long_sums_stay_within_the_bar(cuda, R, P, nq, nkv, hd, own):
     """Hundreds of tiles for every CTA: sums over them in tensor memory, whose additions cut off what does not fit,
     have to be short (a tile of 128 keys takes 8 additions of 2^-24 of the sum per term and product, so the 40 tiles of
